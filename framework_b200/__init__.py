@@ -12,8 +12,8 @@ import importlib
 from . import _lib  # noqa: F401
 
 _OPS = ("Linear", "adamw_step", "add", "add_backward", "bias_gelu", "bias_gelu_backward", "broadcast_shape", "clip_and_step",
-        "device_status", "grad_norm", "launch_count", "matmul", "matmul_backward", "matmul_bias_gelu", "permute",
-        "permute_backward", "plan_describe", "sm_reserve", "softmax", "softmax_backward")
+        "device_status", "grad_norm", "launch_count", "linear_cross_entropy", "linear_cross_entropy_backward", "matmul",
+        "matmul_backward", "matmul_bias_gelu", "muon_step", "orthogonalize", "permute", "permute_backward", "plan_describe", "sm_reserve", "softmax", "softmax_backward")
 
 __all__ = ["DeviceTensor", *_OPS]
 

@@ -17,6 +17,7 @@ ACCUMULATE_C = 1 << 1
 ACCUMULATE_DA = 1 << 2
 ACCUMULATE_DB = 1 << 3
 ACCUMULATE_DBIAS = 1 << 4
+DB_TRANSPOSED = 1 << 5
 FORCE_TENSOR_PATH = 1 << 8
 FORCE_SKINNY_PATH = 1 << 9
 FORCE_PACK = 1 << 10
@@ -74,6 +75,16 @@ _SIGNATURES = {
     "mni_b200_clip_and_step": (C.c_int, [C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float,
                                          C.c_float, C.c_float, C.c_float, C.c_float, C.c_uint32, C.c_float, C.c_void_p,
                                          C.c_void_p]),
+    "mni_b200_linear_cross_entropy_fwd": (C.c_int, [C.POINTER(View), C.POINTER(View), C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                                    C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
+    "mni_b200_linear_cross_entropy_bwd": (C.c_int, [C.POINTER(View), C.POINTER(View), C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32,
+                                                    C.c_void_p]),
+    "mni_b200_orthogonalize": (C.c_int, [C.POINTER(View), C.c_void_p, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float,
+                                         C.c_void_p]),
+    "mni_b200_muon_step": (C.c_int, [C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float,
+                                     C.c_float, C.c_int, C.c_float, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float,
+                                     C.c_void_p]),
     "mni_b200_contiguous": (C.c_int, [C.POINTER(View), C.c_void_p, C.c_void_p]),
     "mni_b200_sm_reserve": (C.c_int, [C.c_int]),
     "mni_b200_workspace_set": (C.c_int, [C.c_void_p, C.c_size_t]),

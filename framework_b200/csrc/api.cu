@@ -12,6 +12,8 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <iterator>
+#include <map>
 #include <mutex>
 #include <string>
 #include <thread>
@@ -113,10 +115,11 @@ struct Arena {
     DeviceState *st = nullptr;
     bool dry = false;
     size_t used = 0;
-    std::vector<std::pair<size_t, size_t>> blocks;   // (offset, bytes) in request order
+    size_t peak = 0;                                 // `used` at its most: a caller may set it back where a step's scratch is free again
     size_t reserve(size_t bytes) {
         const size_t off = used;
         used += (bytes + 255) & ~static_cast<size_t>(255);
+        peak = std::max(peak, used);
         return off;
     }
 };
@@ -1244,6 +1247,264 @@ int bwd_body(Call &c, const mni_b200_view *a, const mni_b200_view *b, const mni_
     return rc;
 }
 
+// ------------------------------------------------------------------ softmax cross entropy of a projection
+struct LossCall {
+    const mni_b200_view *x, *w;
+    const float *bias;
+    Targets targets;
+    int reduction;
+    int64_t M, N, K;
+    int64_t x_shape[MNI_B200_MAX_DIMS];
+};
+
+int check_loss(const mni_b200_view *x, const mni_b200_view *w, const float *bias, const void *targets, int target_bytes, int reduction,
+               LossCall &l) {
+    int rc = check_view(x, "x", 2);
+    if (rc) return rc;
+    rc = check_view(w, "w", 2);
+    if (rc) return rc;
+    if (w->ndim != 2) return fail(MNI_B200_ERR_ARG, "w has %d dims, a matrix is needed", w->ndim);
+    l.x = x;
+    l.w = w;
+    l.bias = bias;
+    l.targets = Targets{targets, target_bytes};
+    l.reduction = reduction;
+    l.K = x->shape[x->ndim - 1];
+    l.N = w->shape[1];
+    if (w->shape[0] != l.K)
+        return fail(MNI_B200_ERR_INNER_DIM, "inner dimensions must match: %lld vs %lld", (long long)l.K, (long long)w->shape[0]);
+    if (l.N == 0 || l.K == 0) return fail(MNI_B200_ERR_ARG, "no classes or no features");
+    l.M = 1;
+    for (int d = 0; d < x->ndim - 1; ++d) {
+        if (x->shape[d] != 0 && l.M > 0x7fffffffLL / x->shape[d]) return fail(MNI_B200_ERR_TOO_LARGE, "more than 2^31-1 rows");
+        l.M *= x->shape[d];
+    }
+    if (target_bytes != 4 && target_bytes != 8) return fail(MNI_B200_ERR_ARG, "targets of %d bytes: 4 or 8 are taken", target_bytes);
+    if (reduction < MNI_B200_REDUCE_NONE || reduction > MNI_B200_REDUCE_MEAN) return fail(MNI_B200_ERR_ARG, "unknown reduction %d", reduction);
+    if (l.M > 0 && !targets) return fail(MNI_B200_ERR_ARG, "targets is null");
+    if ((reinterpret_cast<uintptr_t>(targets) & (target_bytes - 1)) != 0) return fail(MNI_B200_ERR_ARG, "targets are not aligned");
+    return MNI_B200_OK;
+}
+
+// x as a matrix of rows, read in place where its leading dims can be merged, else gathered.
+int rows_of_x(Call &c, const LossCall &l, mni_b200_view &rows) {
+    const mni_b200_view &x = *l.x;
+    rows = mni_b200_view{};
+    rows.ndim = 2;
+    rows.shape[0] = l.M;
+    rows.shape[1] = l.K;
+    int64_t step = 0, span = 0;                    // stride of the rows so far, innermost leading dim first
+    bool merge = true, first = true;
+    for (int d = x.ndim - 2; d >= 0 && merge; --d) {
+        if (x.shape[d] == 1) continue;
+        if (first) step = x.stride[d];
+        else merge = x.stride[d] == span;
+        span = x.stride[d] * x.shape[d];
+        first = false;
+    }
+    if (merge && (l.M == 1 || step > 0)) {
+        rows.ptr = x.ptr;
+        rows.stride[0] = step > 0 ? step : l.K * x.stride[x.ndim - 1];
+        rows.stride[1] = x.stride[x.ndim - 1];
+        return MNI_B200_OK;
+    }
+    const size_t at = c.arena.reserve(static_cast<size_t>(l.M * l.K) * sizeof(float));
+    rows.ptr = c.dry() ? reinterpret_cast<const float *>(static_cast<uintptr_t>(256)) : c.at(at);
+    rows.stride[0] = l.K;
+    rows.stride[1] = 1;
+    if (c.dry()) return MNI_B200_OK;
+    const GatherView job{&x, c.at(at), l.K};
+    return launch_gather(&job, 1, c.stream);
+}
+
+RowsIn rows_in(const LossCall &l) {
+    RowsIn r{};
+    r.ptr = l.x->ptr;
+    r.rows = static_cast<int>(l.M);
+    r.cols = static_cast<int>(l.K);
+    r.nd = l.x->ndim - 1;
+    r.col_stride = l.x->stride[l.x->ndim - 1];
+    for (int d = 0; d < r.nd; ++d) {
+        r.shape[d] = static_cast<int>(l.x->shape[d]);
+        r.stride[d] = l.x->stride[d];
+    }
+    return r;
+}
+
+int loss_fwd_body(Call &c, const LossCall &l, float *loss, float *lse) {
+    if (l.M == 0) return MNI_B200_OK;
+    const int64_t stretches = (l.N + kLogitStretch - 1) / kLogitStretch;
+    if (l.M * stretches > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld classes are too many", (long long)l.M, (long long)l.N);
+    const size_t pairs = c.arena.reserve(static_cast<size_t>(stretches * l.M) * sizeof(float2));
+    const size_t picked = c.arena.reserve(static_cast<size_t>(l.M) * sizeof(float));
+    const size_t sums = c.arena.reserve(loss_sums_bytes(l.M));
+    mni_b200_view x;
+    int rc = rows_of_x(c, l, x);
+    if (rc) return rc;
+    const size_t z_at = c.arena.reserve(static_cast<size_t>(l.M * l.N) * sizeof(float));
+    float *const z = c.dry() ? reinterpret_cast<float *>(static_cast<uintptr_t>(256)) : c.at(z_at);
+    rc = fwd_body(c, &x, l.w, z, l.bias);
+    if (rc || c.dry()) return rc;
+    float2 *const p = reinterpret_cast<float2 *>(c.at(pairs));
+    rc = launch_logit_stats(z, l.M, l.N, l.targets, p, c.at(picked), c.stream);
+    if (rc) return rc;
+    return launch_loss_finish(p, stretches, l.M, l.N, l.targets, c.at(picked), l.reduction, loss, lse, reinterpret_cast<double2 *>(c.at(sums)),
+                              c.stream);
+}
+
+int loss_bwd_body(Call &c, const LossCall &l, const float *lse, const float *grad, float *dx, float *dw, float *dbias) {
+    if (!dx && !dw && !dbias) return MNI_B200_OK;
+    const bool turned = (c.flags & MNI_B200_DB_TRANSPOSED) != 0;
+    if (l.M == 0) {
+        int rc = dw ? zero_or_bias_fill(c, dw, l.K, l.N, nullptr, (c.flags & MNI_B200_ACCUMULATE_DB) != 0) : static_cast<int>(MNI_B200_OK);
+        if (rc == MNI_B200_OK && dbias) rc = zero_or_bias_fill(c, dbias, 1, l.N, nullptr, (c.flags & MNI_B200_ACCUMULATE_DBIAS) != 0);
+        return rc;
+    }
+    const int64_t stretches = (l.N + kLogitStretch - 1) / kLogitStretch;
+    if (l.M * stretches > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld classes are too many", (long long)l.M, (long long)l.N);
+    const size_t count = c.arena.reserve(sizeof(int));
+    const size_t weights = c.arena.reserve(static_cast<size_t>(l.M) * sizeof(float));
+    const size_t copy = c.arena.reserve(static_cast<size_t>(l.M * l.K) * sizeof(float));
+    float *const fake = reinterpret_cast<float *>(static_cast<uintptr_t>(256));
+    mni_b200_view x{};
+    x.ptr = c.dry() ? fake : c.at(copy);
+    x.ndim = 2;
+    x.shape[0] = l.M; x.shape[1] = l.K;
+    x.stride[0] = l.K; x.stride[1] = 1;
+    int rc = MNI_B200_OK;
+    if (!c.dry()) {
+        rc = launch_row_weights(rows_in(l), l.targets, l.reduction, grad, reinterpret_cast<int *>(c.at(count)), c.at(weights), c.at(copy), false,
+                                c.st->sm_count, c.stream);
+        if (rc) return rc;
+    }
+    const size_t z_at = c.arena.reserve(static_cast<size_t>(l.M * l.N) * sizeof(float));
+    mni_b200_view z{};
+    z.ptr = c.dry() ? fake : c.at(z_at);
+    z.ndim = 2;
+    z.shape[0] = l.M; z.shape[1] = l.N;
+    z.stride[0] = l.N; z.stride[1] = 1;
+    const uint32_t flags = c.flags;
+    c.flags = 0;
+    rc = fwd_body(c, &x, l.w, const_cast<float *>(z.ptr), l.bias);
+    if (rc == MNI_B200_OK && !c.dry()) rc = launch_logit_grad(const_cast<float *>(z.ptr), l.M, l.N, l.targets, lse, c.at(weights), c.stream);
+    c.flags = flags & (MNI_B200_ACCUMULATE_DA | MNI_B200_ACCUMULATE_DB | MNI_B200_ACCUMULATE_DBIAS);
+    if (rc == MNI_B200_OK && !turned) rc = bwd_body(c, &x, l.w, &z, dx, dw, dbias);
+    if (rc == MNI_B200_OK && turned) {
+        if (dx || dbias) rc = bwd_body(c, &x, l.w, &z, dx, nullptr, dbias);
+        if (rc == MNI_B200_OK && dw) {             // dw^T = z^T x
+            mni_b200_view zt = z;
+            std::swap(zt.shape[0], zt.shape[1]);
+            std::swap(zt.stride[0], zt.stride[1]);
+            c.flags = (flags & MNI_B200_ACCUMULATE_DB) != 0 ? MNI_B200_ACCUMULATE_C : 0u;
+            rc = fwd_body(c, &zt, &x, dw, nullptr);
+        }
+    }
+    c.flags = flags;
+    return rc;
+}
+
+// ------------------------------------------------------------------ Newton-Schulz updates
+struct MuonMatrix {
+    int64_t rows, cols, index;     // index: of its entry
+};
+struct NewtonSchulz {
+    int steps;
+    float a, b, c;
+};
+
+// The steps on `e`'s normalised updates, in place (e[i].x), one matrix after the other.
+int newton_schulz(Call &c, const NewtonSchulz &ns, const MuonMatrix &m, float *x) {
+    const bool tall = m.rows > m.cols;
+    const int64_t side = std::min(m.rows, m.cols), n = m.rows * m.cols;
+    const size_t mark = c.arena.used;
+    const size_t a_at = c.arena.reserve(static_cast<size_t>(side * side) * 4), q_at = c.arena.reserve(static_cast<size_t>(side * side) * 4),
+                 y_at = c.arena.reserve(static_cast<size_t>(n) * 4);
+    float *const fake = reinterpret_cast<float *>(static_cast<uintptr_t>(256));
+    float *const a = c.dry() ? fake : c.at(a_at), *const q = c.dry() ? fake : c.at(q_at), *const y = c.dry() ? fake : c.at(y_at);
+    auto view = [](float *p, int64_t r, int64_t k, bool turned) {
+        mni_b200_view v{};
+        v.ptr = p;
+        v.ndim = 2;
+        v.shape[0] = turned ? k : r; v.shape[1] = turned ? r : k;
+        v.stride[0] = turned ? 1 : k; v.stride[1] = turned ? k : 1;
+        return v;
+    };
+    const mni_b200_view X = view(x, m.rows, m.cols, false), XT = view(x, m.rows, m.cols, true), A = view(a, side, side, false), Q = view(q, side, side, false);
+    int rc = MNI_B200_OK;
+    const size_t inner = c.arena.used;
+    for (int s = 0; s < ns.steps && rc == MNI_B200_OK; ++s) {
+        c.arena.used = inner;
+        rc = tall ? fwd_body(c, &XT, &X, a, nullptr) : fwd_body(c, &X, &XT, a, nullptr);
+        if (rc == MNI_B200_OK) rc = fwd_body(c, &A, &A, q, nullptr);
+        if (rc == MNI_B200_OK && !c.dry()) rc = launch_combine(a, q, q, side * side, ns.b, ns.c, c.stream);
+        if (rc == MNI_B200_OK) rc = tall ? fwd_body(c, &X, &Q, y, nullptr) : fwd_body(c, &Q, &X, y, nullptr);
+        if (rc == MNI_B200_OK && !c.dry()) rc = launch_combine(x, y, x, n, ns.a, 1.f, c.stream);
+        if (c.dry()) break;
+    }
+    c.arena.used = mark;
+    return rc;
+}
+
+int muon_body(Call &c, std::vector<MuonEntry> &e, const std::vector<MuonMatrix> &shapes, const NewtonSchulz &ns, float mu, bool nesterov, float eps,
+              float decay, bool scratch_x) {
+    const int64_t count = static_cast<int64_t>(e.size());
+    const size_t partial = c.arena.reserve(muon_partial_bytes(e.data(), count));
+    if (scratch_x)
+        for (MuonEntry &m : e) {
+            const size_t at = c.arena.reserve(static_cast<size_t>(m.n) * sizeof(float));
+            m.x = c.dry() ? reinterpret_cast<float *>(static_cast<uintptr_t>(256)) : c.at(at);
+        }
+    int rc = MNI_B200_OK;
+    if (!c.dry()) rc = launch_muon_start(e.data(), count, mu, nesterov, eps, reinterpret_cast<double *>(c.at(partial)), c.stream);
+    for (int64_t i = 0; i < count && rc == MNI_B200_OK; ++i)
+        if (e[i].n) rc = newton_schulz(c, ns, shapes[i], e[i].x);
+    if (rc == MNI_B200_OK && !c.dry() && scratch_x) rc = launch_muon_update(e.data(), count, decay, c.stream);
+    return rc;
+}
+
+// Stretches of memory, to find whether any is touched twice.
+struct Touched {
+    std::map<uintptr_t, uintptr_t> at;             // begin -> end, disjoint or the same stretch again
+    static std::pair<uintptr_t, uintptr_t> span(const float *p, int64_t n) {
+        const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+        return {b, b + static_cast<uintptr_t>(n) * sizeof(float)};
+    }
+    bool meets(const float *p, int64_t n) const {
+        const auto s = span(p, n);
+        auto next = at.lower_bound(s.second);      // the first that begins behind it; the one before may reach into it
+        return next != at.begin() && std::prev(next)->second > s.first;
+    }
+    void add(const float *p, int64_t n) {          // merged with what it meets
+        auto s = span(p, n);
+        auto it = at.lower_bound(s.second);
+        while (it != at.begin() && std::prev(it)->second > s.first) {
+            it = std::prev(it);
+            s.first = std::min(s.first, it->first);
+            s.second = std::max(s.second, it->second);
+            it = at.erase(it);
+        }
+        at.emplace(s.first, s.second);
+    }
+};
+bool share_memory(const float *p, const float *q, int64_t n) {
+    const auto a = Touched::span(p, n), b = Touched::span(q, n);
+    return a.first < b.second && b.first < a.second;
+}
+
+int check_newton_schulz(int steps, float a, float b, float c, float eps, NewtonSchulz &ns) {
+    if (steps < 0 || steps > 100) return fail(MNI_B200_ERR_ARG, "%d steps", steps);
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return fail(MNI_B200_ERR_ARG, "coefficients must be finite");
+    if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(MNI_B200_ERR_ARG, "eps must be zero or more");
+    ns = NewtonSchulz{steps, a, b, c};
+    return MNI_B200_OK;
+}
+int check_matrix(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 0) return fail(MNI_B200_ERR_ARG, "negative extent");
+    if (rows > 0x7fffffffLL || cols > 0x7fffffffLL || (rows > 0 && cols > (1LL << 38) / rows))
+        return fail(MNI_B200_ERR_TOO_LARGE, "a matrix of %lld x %lld is too large", (long long)rows, (long long)cols);
+    return MNI_B200_OK;
+}
+
 // Runs `body` twice: a dry pass that sizes the scratch, then the real pass.
 template <class Body>
 int with_scratch(uint32_t flags, void *stream, Body body) {
@@ -1264,7 +1525,7 @@ int with_scratch(uint32_t flags, void *stream, Body body) {
         dry.st = st; dry.arena.st = st; dry.arena.dry = true; dry.stream = static_cast<cudaStream_t>(stream); dry.flags = flags;
         rc = body(dry);
         if (rc) return rc;
-        sized = dry.arena.used;
+        sized = dry.arena.peak;
         if (sized == 0) break;
         // Not what would have to be allocated in a capture, which that would end, nor what could not be had before.
         if (dry.used_half && !st->user_ws && sized > st->ws_bytes && (capturing || scratch_refused(*st, sized))) {
@@ -1281,8 +1542,8 @@ int with_scratch(uint32_t flags, void *stream, Body body) {
     rc = body(real);
     // Both passes must have planned the same launches: a real pass that asked for more scratch than was sized
     // would have written past it.
-    if (rc == MNI_B200_OK && real.arena.used > sized)
-        return fail(MNI_B200_ERR_WORKSPACE, "internal: the call used %zu bytes of scratch, %zu were sized", real.arena.used, sized);
+    if (rc == MNI_B200_OK && real.arena.peak > sized)
+        return fail(MNI_B200_ERR_WORKSPACE, "internal: the call used %zu bytes of scratch, %zu were sized", real.arena.peak, sized);
     return rc;
 }
 
@@ -1552,6 +1813,119 @@ int mni_b200_clip_and_step(int64_t count, float *const *params, float *const *ms
     const int waited = lease.wait(s);
     if (rc || waited) return rc ? rc : waited;
     *norm = sqrtf(static_cast<float>(lease.slot->sumsq));
+    return MNI_B200_OK;
+}
+
+int mni_b200_linear_cross_entropy_fwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias, const void *targets,
+                                      int target_bytes, int reduction, float *loss, float *lse, uint32_t flags, void *stream) {
+    LossCall l;
+    int rc = check_loss(x, w, bias, targets, target_bytes, reduction, l);
+    if (rc) return rc;
+    if (flags != 0) return fail(MNI_B200_ERR_ARG, "flags 0x%x are not taken here", flags);
+    if ((l.M > 0 && !lse) || ((l.M > 0 || reduction != MNI_B200_REDUCE_NONE) && !loss)) return fail(MNI_B200_ERR_ARG, "loss or lse is null");
+    if (l.M == 0 && reduction != MNI_B200_REDUCE_NONE) {
+        DeviceState *st = nullptr;
+        rc = device_state(&st);
+        if (rc) return rc;
+        // the sum over no rows; as a mean 0 / 0 (an f32 of all ones is a NaN)
+        MNI_CUDA(cudaMemsetAsync(loss, reduction == MNI_B200_REDUCE_MEAN ? 0xff : 0, sizeof(float), static_cast<cudaStream_t>(stream)));
+        return MNI_B200_OK;
+    }
+    return with_scratch(flags, stream, [&](Call &call) { return loss_fwd_body(call, l, loss, lse); });
+}
+
+int mni_b200_linear_cross_entropy_bwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias, const void *targets,
+                                      int target_bytes, int reduction, const float *lse, const float *grad, float *dx, float *dw,
+                                      float *dbias, uint32_t flags, void *stream) {
+    LossCall l;
+    int rc = check_loss(x, w, bias, targets, target_bytes, reduction, l);
+    if (rc) return rc;
+    constexpr uint32_t kTaken = MNI_B200_ACCUMULATE_DA | MNI_B200_ACCUMULATE_DB | MNI_B200_ACCUMULATE_DBIAS | MNI_B200_DB_TRANSPOSED;
+    if ((flags & ~kTaken) != 0) return fail(MNI_B200_ERR_ARG, "flags 0x%x are not taken here", flags & ~kTaken);
+    if (l.M > 0 && (!lse || !grad)) return fail(MNI_B200_ERR_ARG, "lse or grad is null");
+    return with_scratch(flags, stream, [&](Call &call) { return loss_bwd_body(call, l, lse, grad, dx, dw, dbias); });
+}
+
+int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float a, float b, float c, float eps, void *stream) {
+    int rc = check_view(g, "g", 2);
+    if (rc) return rc;
+    NewtonSchulz ns;
+    rc = check_newton_schulz(steps, a, b, c, eps, ns);
+    if (rc) return rc;
+    const int64_t rows = g->shape[g->ndim - 2], cols = g->shape[g->ndim - 1], batch = prod(g->shape, g->ndim - 2);
+    rc = check_matrix(rows, cols);
+    if (rc) return rc;
+    if (batch * rows * cols == 0) return MNI_B200_OK;
+    if (batch > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "more than 2^31-1 matrices");
+    if (!out) return fail(MNI_B200_ERR_ARG, "out is null");
+    return with_scratch(0, stream, [&](Call &call) -> int {
+        const float *src = g->ptr;
+        bool packed = true;
+        int64_t acc = 1;
+        for (int d = g->ndim - 1; d >= 0; --d) {
+            packed = packed && (g->shape[d] == 1 || g->stride[d] == acc);
+            acc *= g->shape[d];
+        }
+        if (!packed) {                             // into `out`, which is normalised in place
+            if (!call.dry()) {
+                const GatherView job{g, out, cols};
+                const int r = launch_gather(&job, 1, call.stream);
+                if (r) return r;
+            }
+            src = out;
+        }
+        std::vector<MuonEntry> e;
+        std::vector<MuonMatrix> shapes;
+        for (int64_t i = 0; i < batch; ++i) {
+            e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, rows * cols, 0.f});
+            shapes.push_back(MuonMatrix{rows, cols, i});
+        }
+        return muon_body(call, e, shapes, ns, 0.f, false, eps, 1.f, false);
+    });
+}
+
+int mni_b200_muon_step(int64_t count, float *const *params, float *const *momenta, const float *const *grads, const int64_t *rows,
+                       const int64_t *cols, const float *scales, float lr, float momentum, int nesterov, float weight_decay, int steps,
+                       float a, float b, float c, float eps, void *stream) {
+    if (count < 0) return fail(MNI_B200_ERR_ARG, "negative count");
+    if (count > 0 && (!params || !momenta || !grads || !rows || !cols || !scales)) return fail(MNI_B200_ERR_ARG, "null pointer");
+    NewtonSchulz ns;
+    int rc = check_newton_schulz(steps, a, b, c, eps, ns);
+    if (rc) return rc;
+    std::vector<MuonEntry> e;
+    std::vector<MuonMatrix> shapes;
+    for (int64_t i = 0; i < count; ++i) {
+        rc = check_matrix(rows[i], cols[i]);
+        if (rc) return rc;
+        const int64_t n = rows[i] * cols[i];
+        if (n == 0) continue;
+        if (!params[i] || !momenta[i] || !grads[i]) return fail(MNI_B200_ERR_ARG, "null pointer");
+        if (share_memory(params[i], momenta[i], n) || share_memory(params[i], grads[i], n) || share_memory(momenta[i], grads[i], n))
+            return fail(MNI_B200_ERR_ARG, "entry %lld: param, momentum and grad share memory", (long long)i);
+        e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, n, lr * scales[i]});
+        shapes.push_back(MuonMatrix{rows[i], cols[i], i});
+    }
+    // Entries that share memory with one before them begin another round, which starts from what that one left.
+    for (size_t first = 0; first < e.size();) {
+        Touched written, read;
+        size_t end = first;
+        for (; end < e.size(); ++end) {
+            const MuonEntry &m = e[end];
+            if (written.meets(m.param, m.n) || written.meets(m.momentum, m.n) || written.meets(m.grad, m.n) || read.meets(m.param, m.n) ||
+                read.meets(m.momentum, m.n))
+                break;
+            written.add(m.param, m.n);
+            written.add(m.momentum, m.n);
+            read.add(m.grad, m.n);
+        }
+        std::vector<MuonEntry> round(e.begin() + first, e.begin() + end);
+        const std::vector<MuonMatrix> sizes(shapes.begin() + first, shapes.begin() + end);
+        rc = with_scratch(0, stream, [&](Call &call) -> int {
+            return muon_body(call, round, sizes, ns, momentum, nesterov != 0, eps, 1.f - lr * weight_decay, true);
+        });
+        if (rc) return rc;
+        first = end;
+    }
     return MNI_B200_OK;
 }
 

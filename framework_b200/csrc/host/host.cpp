@@ -16,6 +16,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <new>
 #include <vector>
 
@@ -52,6 +54,10 @@ struct Api {
     decltype(&mni_b200_contiguous) contiguous;
     decltype(&mni_b200_grad_norm_sq) grad_norm_sq;
     decltype(&mni_b200_clip_and_step) clip_and_step;
+    decltype(&mni_b200_linear_cross_entropy_fwd) linear_cross_entropy_fwd;
+    decltype(&mni_b200_linear_cross_entropy_bwd) linear_cross_entropy_bwd;
+    decltype(&mni_b200_orthogonalize) orthogonalize;
+    decltype(&mni_b200_muon_step) muon_step;
 };
 Api g_api;
 bool g_bound = false;
@@ -853,6 +859,222 @@ PyObject *op_clip_and_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     return PyFloat_FromDouble(static_cast<double>(norm));
 }
 
+// ------------------------------------------------------------------ cross entropy of a projection
+// What the two operators check alike: x [.., K], weight [K, N], whole-number targets of x's leading shape, bias [N] or None.
+struct LossOperands {
+    TensorObj *x = nullptr, *w = nullptr, *bias = nullptr;
+    at::Tensor targets;
+    int target_bytes = 0, reduction = 0;
+    Dims rows;
+    int64_t k = 0, n = 0;
+    bool parse(PyObject *px, PyObject *pw, PyObject *pt, PyObject *pb, PyObject *pr) {
+        x = as_tensor(px, "x");
+        w = x ? as_tensor(pw, "weight") : nullptr;
+        if (!w) return false;
+        if (x->shape.size() < 2 || w->shape.size() != 2 || x->shape.back() != w->shape[0]) {
+            PyObject *have = tuple_of(x->shape), *of = tuple_of(w->shape);
+            if (have && of) PyErr_Format(PyExc_ValueError, "x must be [.., K] with at least 2 dims and weight [K, N]: %R and %R", have, of);
+            Py_XDECREF(have);
+            Py_XDECREF(of);
+            return false;
+        }
+        k = w->shape[0];
+        n = w->shape[1];
+        rows.assign(x->shape.begin(), x->shape.end() - 1);
+        if (!THPVariable_Check(pt)) { PyErr_SetString(PyExc_TypeError, "targets must be a torch tensor of int32 or int64"); return false; }
+        targets = THPVariable_Unpack(pt);
+        if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt) {
+            PyErr_SetString(PyExc_TypeError, "targets must be a torch tensor of int32 or int64");
+            return false;
+        }
+        target_bytes = targets.scalar_type() == at::kLong ? 8 : 4;
+        bool fits = static_cast<size_t>(targets.dim()) == rows.size();
+        for (size_t i = 0; fits && i < rows.size(); ++i) fits = targets.size(static_cast<int64_t>(i)) == rows[i];
+        if (!fits) { PyErr_SetString(PyExc_ValueError, "targets must have x's shape without its last dim"); return false; }
+        if (targets.device() != x->flat.device() || w->flat.device() != x->flat.device()) {
+            PyErr_SetString(PyExc_ValueError, "x, weight and targets must be on one device");
+            return false;
+        }
+        targets = targets.contiguous();
+        if (pb != Py_None) {
+            bias = as_tensor(pb, "bias");
+            if (!bias) return false;
+            if (!vector_of(bias, n) || !bias->contiguous) { PyErr_SetString(PyExc_ValueError, "bias must be a contiguous [N] vector"); return false; }
+        }
+        reduction = static_cast<int>(PyLong_AsLong(pr));
+        return !PyErr_Occurred();
+    }
+};
+
+// linear_cross_entropy(x, weight, targets, bias, reduction) -> (loss, lse)
+PyObject *op_linear_cross_entropy(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    ARGS(5, "linear_cross_entropy(x, weight, targets, bias, reduction)");
+    LossOperands o;
+    if (!o.parse(args[0], args[1], args[2], args[3], args[4])) return nullptr;
+    const at::Device device = o.x->flat.device();
+    Ref loss(new_tensor(o.reduction == MNI_B200_REDUCE_NONE ? o.rows : Dims{1}, device)), lse(loss ? new_tensor(o.rows, device) : nullptr);
+    if (!loss || !lse) return nullptr;
+    mni_b200_view vx, vw;
+    if (!make_view(o.x, vx) || !make_view(o.w, vw)) return nullptr;
+    const float *bias = o.bias ? data(o.bias) : nullptr;
+    float *pl = data(loss.t), *ps = data(lse.t);
+    const void *targets = o.targets.data_ptr();
+    void *stream = current_stream();
+    CALL(g_api.linear_cross_entropy_fwd(&vx, &vw, bias, targets, o.target_bytes, o.reduction, pl, ps, 0, stream));
+    return pair_of(loss, lse);
+}
+
+// linear_cross_entropy_backward(grad, x, weight, targets, lse, bias, reduction, flags, need_dx, need_dw, want_dbias, dx, dw, dbias)
+PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    ARGS(14, "linear_cross_entropy_backward(grad, x, weight, targets, lse, bias, reduction, flags, need_dx, need_dw, want_dbias, dx, dw, dbias)");
+    uint32_t flags;
+    bool need_dx, need_dw, want_dbias;
+    if (!parse_flags(args[7], flags) || !parse_truth(args[8], need_dx) || !parse_truth(args[9], need_dw) || !parse_truth(args[10], want_dbias))
+        return nullptr;
+    LossOperands o;
+    if (!o.parse(args[1], args[2], args[3], args[5], args[6])) return nullptr;
+    TENSOR(g0, 0, "grad");
+    TENSOR(s0, 4, "lse");
+    if (s0->shape != o.rows) { PyErr_SetString(PyExc_ValueError, "lse must have x's shape without its last dim"); return nullptr; }
+    if (o.reduction == MNI_B200_REDUCE_NONE ? g0->shape != o.rows : numel(g0->shape) != 1) {
+        PyErr_SetString(PyExc_ValueError, "grad must have the loss's shape");
+        return nullptr;
+    }
+    Ref g(contiguous_of(g0)), lse(g ? contiguous_of(s0) : nullptr);
+    if (!g || !lse) return nullptr;
+    const at::Device device = o.x->flat.device();
+    Ref dx, dw, dbias;
+    if (need_dx && !output(args[11], o.x->shape, device, "dx", dx)) return nullptr;
+    // a weight seen through a transposing view has its gradient laid out as it is stored itself
+    const Dims shape{o.k, o.n}, stored{o.n, o.k};
+    bool turned = o.k > 1 && o.n > 1 && o.w->stride[0] == 1 && o.w->stride[1] != 1;
+    if (need_dw && args[12] == Py_None) {
+        dw.reset(new_tensor(turned ? stored : shape, device));
+        if (dw && turned) dw.reset(reinterpret_cast<TensorObj *>(permuted(dw.t, Dims{1, 0})));
+        if (!dw) return nullptr;
+    } else if (need_dw) {
+        if (!output(args[12], shape, device, "dw", dw)) return nullptr;
+        turned = !dw.t->contiguous;
+    }
+    if (want_dbias && !output(args[13], Dims{o.n}, device, "dbias", dbias)) return nullptr;
+    if ((dx && (dx.t->shape != o.x->shape || !dx.t->contiguous)) || (dbias && (!vector_of(dbias.t, o.n) || !dbias.t->contiguous)) ||
+        (dw && (dw.t->shape != shape || (turned && !(dw.t->stride[0] == 1 && dw.t->stride[1] == o.k))))) {
+        PyErr_SetString(PyExc_ValueError, "dx and dbias must be contiguous, dw contiguous or the transposing view of a contiguous [N, K]");
+        return nullptr;
+    }
+    mni_b200_view vx, vw;
+    if (!make_view(o.x, vx) || !make_view(o.w, vw)) return nullptr;
+    const float *bias = o.bias ? data(o.bias) : nullptr, *pl = data(lse.t), *pg = data(g.t);
+    float *pdx = dx ? data(dx.t) : nullptr, *pdw = dw ? data(dw.t) : nullptr, *pdb = dbias ? data(dbias.t) : nullptr;
+    const void *targets = o.targets.data_ptr();
+    if (turned && need_dw) flags |= MNI_B200_DB_TRANSPOSED;
+    void *stream = current_stream();
+    CALL(g_api.linear_cross_entropy_bwd(&vx, &vw, bias, targets, o.target_bytes, o.reduction, pl, pg, pdx, pdw, pdb, flags, stream));
+    PyObject *results[3];
+    Ref *mine[3] = {&dx, &dw, &dbias};
+    const int count = want_dbias ? 3 : 2;
+    for (int i = 0; i < count; ++i) results[i] = *mine[i] ? mine[i]->release() : (Py_INCREF(args[11 + i]), args[11 + i]);
+    PyObject *tuple = PyTuple_New(count);
+    for (int i = 0; i < count; ++i) {
+        if (tuple) PyTuple_SET_ITEM(tuple, i, results[i]);
+        else Py_DECREF(results[i]);
+    }
+    return tuple;
+}
+
+// ------------------------------------------------------------------ Newton-Schulz updates
+// (steps, a, b, c, eps) from args[0..4]
+struct NewtonSchulzArgs {
+    int steps;
+    float v[4];
+    bool parse(PyObject *const *args) {
+        const long given = PyLong_AsLong(args[0]);
+        steps = static_cast<int>(std::max<long>(-1, std::min<long>(given, 1 << 20)));
+        for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(PyFloat_AsDouble(args[1 + i]));
+        return !PyErr_Occurred();
+    }
+};
+
+// orthogonalize(g, steps, a, b, c, eps)
+PyObject *op_orthogonalize(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    ARGS(6, "orthogonalize(g, steps, a, b, c, eps)");
+    TENSOR(g, 0, "g");
+    NewtonSchulzArgs ns;
+    if (!ns.parse(args + 1)) return nullptr;
+    if (g->shape.size() < 2) { PyErr_SetString(PyExc_ValueError, "orthogonalize requires at least 2D tensors"); return nullptr; }
+    Ref out(new_tensor(g->shape, g->flat.device()));
+    if (!out) return nullptr;
+    mni_b200_view vg;
+    if (!make_view(g, vg)) return nullptr;
+    float *po = data(out.t);
+    void *stream = current_stream();
+    CALL(g_api.orthogonalize(&vg, po, ns.steps, ns.v[0], ns.v[1], ns.v[2], ns.v[3], stream));
+    return out.release();
+}
+
+// muon_step(params, momenta, grads, scale, lr, momentum, nesterov, weight_decay, steps, a, b, c, eps).  scale: 0 by shape
+// (sqrt(max(1, cols / rows))), 1 by size (0.2 sqrt(max(rows, cols))), or a float for all.
+PyObject *op_muon_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    ARGS(13, "muon_step(params, momenta, grads, scale, lr, momentum, nesterov, weight_decay, steps, a, b, c, eps)");
+    const double lr = PyFloat_AsDouble(args[4]), mu = PyFloat_AsDouble(args[5]), decay = PyFloat_AsDouble(args[7]);
+    const bool by_rule = PyLong_Check(args[3]);
+    const double given = by_rule ? 0.0 : PyFloat_AsDouble(args[3]);
+    const long rule = by_rule ? PyLong_AsLong(args[3]) : -1;
+    bool nesterov;
+    NewtonSchulzArgs ns;
+    if (PyErr_Occurred() || !parse_truth(args[6], nesterov) || !ns.parse(args + 8)) return nullptr;
+    PyObject *lists[3] = {nullptr, nullptr, nullptr};
+    struct Drop {
+        PyObject **l;
+        ~Drop() { for (int i = 0; i < 3; ++i) Py_XDECREF(l[i]); }
+    } drop{lists};
+    for (int i = 0; i < 3; ++i) {
+        lists[i] = PySequence_Fast(args[i], "expected a sequence of tensors");
+        if (!lists[i]) return nullptr;
+    }
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(lists[0]);
+    if (PySequence_Fast_GET_SIZE(lists[1]) != count || PySequence_Fast_GET_SIZE(lists[2]) != count) {
+        PyErr_SetString(PyExc_ValueError, "params, momenta and grads must have the same length");
+        return nullptr;
+    }
+    std::vector<float *> p, m;
+    std::vector<const float *> g;
+    std::vector<int64_t> rows, cols;
+    std::vector<float> scales;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        TensorObj *t[3];
+        for (int k = 0; k < 3; ++k) {
+            t[k] = as_tensor(PySequence_Fast_GET_ITEM(lists[k], i), "every element");
+            if (!t[k]) return nullptr;
+            if (!t[k]->contiguous) { PyErr_SetString(PyExc_ValueError, "muon_step needs contiguous tensors"); return nullptr; }
+        }
+        const Dims &shape = t[0]->shape;
+        if (t[1]->shape != shape || t[2]->shape != shape) {
+            PyErr_SetString(PyExc_ValueError, "param, momentum and grad must have the same shape");
+            return nullptr;
+        }
+        if (shape.size() < 2) { PyErr_SetString(PyExc_ValueError, "muon_step takes matrices: at least 2D tensors"); return nullptr; }
+        // leading dims: that many matrices
+        const int64_t r = shape[shape.size() - 2], c = shape.back(), each = r * c, batch = each ? numel(shape) / each : 0;
+        const double scale = rule == 0 ? std::sqrt(std::max(1.0, static_cast<double>(c) / static_cast<double>(std::max<int64_t>(r, 1))))
+                             : rule == 1 ? 0.2 * std::sqrt(static_cast<double>(std::max(r, c)))
+                                         : given;
+        for (int64_t b = 0; b < batch; ++b) {
+            p.push_back(data(t[0]) + b * each);
+            m.push_back(data(t[1]) + b * each);
+            g.push_back(data(t[2]) + b * each);
+            rows.push_back(r);
+            cols.push_back(c);
+            scales.push_back(static_cast<float>(scale));
+        }
+    }
+    void *stream = current_stream();
+    CALL(g_api.muon_step(static_cast<int64_t>(p.size()), p.data(), m.data(), g.data(), rows.data(), cols.data(), scales.data(),
+                         static_cast<float>(lr), static_cast<float>(mu), nesterov ? 1 : 0, static_cast<float>(decay), ns.steps, ns.v[0], ns.v[1],
+                         ns.v[2], ns.v[3], stream));
+    Py_RETURN_NONE;
+}
+
 // ------------------------------------------------------------------ module
 // setup(cls, loader, raise_status, check_shapes): the Python side of the bindings
 PyObject *setup(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -874,7 +1096,8 @@ PyObject *bind(PyObject *, PyObject *table) {
 #define ENTRY(field) {"mni_b200_" #field, reinterpret_cast<void **>(&g_api.field)}
         ENTRY(matmul_fwd), ENTRY(matmul_bwd), ENTRY(matmul_bias_gelu_fwd), ENTRY(add_bias), ENTRY(add_bias_bwd),
         ENTRY(bias_gelu), ENTRY(bias_gelu_bwd), ENTRY(softmax_fwd), ENTRY(softmax_bwd), ENTRY(contiguous),
-        ENTRY(grad_norm_sq), ENTRY(clip_and_step),
+        ENTRY(grad_norm_sq), ENTRY(clip_and_step), ENTRY(linear_cross_entropy_fwd), ENTRY(linear_cross_entropy_bwd),
+        ENTRY(orthogonalize), ENTRY(muon_step),
 #undef ENTRY
     };
     for (auto &e : entries) {
@@ -910,6 +1133,10 @@ PyMethodDef module_methods[] = {
     FAST("permute_backward", op_permute_backward, "ops.permute_backward"),
     FAST("grad_norm_sq", op_grad_norm_sq, "squared global gradient norm into a device double"),
     FAST("clip_and_step", op_clip_and_step, "ops.clip_and_step"),
+    FAST("linear_cross_entropy", op_linear_cross_entropy, "ops.linear_cross_entropy"),
+    FAST("linear_cross_entropy_backward", op_linear_cross_entropy_backward, "ops.linear_cross_entropy_backward"),
+    FAST("orthogonalize", op_orthogonalize, "ops.orthogonalize"),
+    FAST("muon_step", op_muon_step, "ops.muon_step"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "native host side of the operator interface", -1, module_methods,
                           nullptr, nullptr, nullptr, nullptr};

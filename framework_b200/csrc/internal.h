@@ -311,6 +311,58 @@ size_t half_columns_bytes(const HalfView &first, int blocks);
 // planes: 3, for products in full precision (f16 hi and lo, or three bf16), or 2, for single-pass ones (f16 hi, or two bf16)
 int launch_split_half(const HalfView *views, int count, int planes, unsigned int *status, int blocks, const HalfColumns &sums,
                       cudaStream_t stream);
+// Softmax cross entropy of a projection (loss.cu).
+struct Targets {
+    const void *ptr;               // whole numbers of `bytes` bytes (4 or 8), one per row; below zero: the row is left out
+    int bytes;
+};
+// The rows of a tensor of up to 8 dims, its last dim the columns.
+struct RowsIn {
+    const float *ptr;
+    int rows, cols, nd;            // nd leading dims, outermost first
+    long long col_stride;
+    int shape[7];
+    long long stride[7];
+#ifdef __CUDACC__
+    __device__ long long offset(int row) const {
+        long long at = 0;
+        for (int d = nd - 1; d >= 0; --d) {
+            at += (row % shape[d]) * stride[d];
+            row /= shape[d];
+        }
+        return at;
+    }
+#endif
+};
+constexpr int kLogitStretch = 2048;    // logits of a row that one block joins into a pair (maximum, sum of exponentials)
+// pairs[stretch][row]; at_target[row] is written where this call's classes include the target
+int launch_logit_stats(const float *z, int64_t rows, int64_t n, const Targets &targets, float2 *pairs, float *at_target, cudaStream_t stream);
+size_t loss_sums_bytes(int64_t rows);
+int launch_loss_finish(const float2 *pairs, int64_t parts, int64_t rows, int64_t classes, const Targets &targets, const float *at_target,
+                       int reduction, float *loss, float *lse, double2 *sums, cudaStream_t stream);
+// weights[row] = the row's share in the reduced loss times its gradient; copy (may be null): x, rows left out as zeros, the others
+// multiplied by their weights if `scaled`
+int launch_row_weights(const RowsIn &x, const Targets &targets, int reduction, const float *grad, int *count, float *weights, float *copy,
+                       bool scaled, int sm_count, cudaStream_t stream);
+// z -> weights * (exp(z - lse) - [class = target])
+int launch_logit_grad(float *z, int64_t rows, int64_t n, const Targets &targets, const float *lse, const float *weights, cudaStream_t stream);
+
+// Newton-Schulz updates (muon.cu).
+struct MuonEntry {
+    float *param, *momentum;       // null for a matrix that is only made orthogonal
+    const float *grad;
+    float *x;                      // the normalised update
+    int64_t n;
+    float scale;                   // of the update (learning rate included)
+};
+// momentum = mu * momentum + grad, and the sums of squares of the update u = grad + mu * momentum (nesterov) or momentum, or
+// grad where there is no momentum; then x = u / (norm + eps)
+size_t muon_partial_bytes(const MuonEntry *e, int64_t count);
+int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, cudaStream_t stream);
+// param = decay * param - scale * x
+int launch_muon_update(const MuonEntry *e, int64_t count, float decay, cudaStream_t stream);
+// out = alpha * x + beta * y
+int launch_combine(const float *x, const float *y, float *out, int64_t n, float alpha, float beta, cudaStream_t stream);
 // device-side utils::unbroadcast: out[orig] (+)= sum over broadcast dims of grad[gshape]
 int launch_unbroadcast(const float *grad, const int64_t *gshape, int gnd, const int64_t *oshape, int ond,
                        float *out, bool accumulate, cudaStream_t stream);

@@ -1,0 +1,292 @@
+// Softmax cross entropy of a projection, z = x.w (+ bias), without its logits in the caller's memory, and its gradient.
+//
+//   lse[r] = log sum_j exp z[r, j],  loss[r] = lse[r] - z[r, t[r]],  d[r, j] = exp(z[r, j] - lse[r]) - [j = t[r]]
+//   dx = diag(g) d w^T,  dw = (diag(g) x)^T d,  dbias = sum_r g[r] d[r, :]
+//
+// A row's sum of exponentials is kept as pairs (m, s), the sum being s * exp(m): one pair for each stretch of classes, joined by
+// loss_finish_kernel.  m is the stretch's maximum; a stretch of nothing but -inf has s = 0 and m = -inf, one with +inf has
+// m = +inf (and lse = +inf), NaN stays in s.  Sums of exponentials are in f32 over a stretch and in f32 over its stretches,
+// sums over rows in f64, both in a fixed order.
+//
+// A target below zero leaves its row out: loss 0, no gradient, whatever the row of x holds.  One that is no class makes the
+// row's loss, and with it the gradients, NaN: a mistake that shows, where a check would have to wait for the device.
+#include "internal.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mni {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kStretch = kLogitStretch;            // classes per block of the kernel for logits in memory
+constexpr int kPer = kStretch / kThreads;
+
+__device__ __forceinline__ long long target_at(const Targets &t, long long row) {
+    return t.bytes == 8 ? static_cast<const long long *>(t.ptr)[row] : static_cast<const int *>(t.ptr)[row];
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// s * exp(m - to), 0 where there is nothing to add; NaN in s stays.
+__device__ __forceinline__ float rescaled(float m, float s, float to) {
+    return m == to ? s : (m == -INFINITY ? s : s * expf(m - to));
+}
+
+// Pairs (m, s) of stretches of the logits z[rows, n] of classes first .. first + n, and the targets' logits.  One block per
+// row and stretch, whose elements stay in registers between the maximum and the sum.  Bound by memory, 4 bytes an element.
+__global__ void __launch_bounds__(kThreads)
+logit_stats_kernel(const float *__restrict__ z, int rows, int n, FastDiv stretches, Targets targets, float2 *__restrict__ pairs,
+                   float *__restrict__ at_target) {
+    __shared__ float red[8];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int row = fd_div(blockIdx.x, stretches), stretch = static_cast<int>(blockIdx.x - row * stretches.d), c0 = stretch * kStretch;
+    const float *src = z + static_cast<long long>(row) * n;
+    float v[kPer];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c = c0 + i * kThreads + threadIdx.x;
+        v[i] = c < n ? src[c] : -INFINITY;
+        m = fmaxf(m, v[i]);
+    }
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) m = fmaxf(m, red[w]);
+    const float shift = isinf(m) ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s += expf(v[i] - shift);
+    s = warp_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = red[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += red[w];
+        pairs[static_cast<long long>(stretch) * rows + row] = make_float2(m, s);
+        const long long t = target_at(targets, row);
+        if (t >= c0 && t < min(n, c0 + kStretch)) at_target[row] = src[t];
+    }
+}
+
+// Joins the pairs of 32 rows a block, `parts` of them each, eight warps taking every eighth.  sums: a pair (sum of losses, rows
+// counted) per block; with one block the reduced loss is written here, else by loss_sum_kernel.
+__global__ void __launch_bounds__(kThreads)
+loss_finish_kernel(const float2 *__restrict__ pairs, int parts, int rows, int classes, Targets targets, const float *__restrict__ at_target,
+                   int reduction, float *__restrict__ loss, float *__restrict__ lse, double2 *__restrict__ sums) {
+    __shared__ float2 part[8][32];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x * 32 + lane;
+    float m = -INFINITY, s = 0.f;
+    if (row < rows) {
+        for (int p0 = warp; p0 < parts; p0 += 64) {            // eight loads on their way together
+            float2 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int p = p0 + 8 * u;
+                x[u] = p < parts ? __ldcg(pairs + static_cast<long long>(p) * rows + row) : make_float2(-INFINITY, 0.f);
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+            s = rescaled(m, s, top);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += rescaled(x[u].x, x[u].y, top);
+            m = top;
+        }
+    }
+    part[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    if (warp != 0) return;
+    double l = 0.0;
+    int counted = 0;
+    if (row < rows) {
+        float top = m;
+#pragma unroll
+        for (int w = 1; w < 8; ++w) top = fmaxf(top, part[w][lane].x);
+        s = rescaled(m, s, top);
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += rescaled(part[w][lane].x, part[w][lane].y, top);
+        const float total = top == -INFINITY ? logf(s) : top + logf(s);
+        lse[row] = total;
+        const long long t = target_at(targets, row);
+        float one = 0.f;
+        if (t >= 0) {
+            one = t < classes ? total - __ldcg(at_target + row) : NAN;
+            counted = 1;
+            l = one;
+        }
+        if (reduction == 0) loss[row] = one;
+    }
+    if (reduction == 0) return;
+    l = warp_sum(l);
+    counted = __reduce_add_sync(0xffffffffu, counted);
+    if (lane == 0) {
+        if (gridDim.x == 1) loss[0] = static_cast<float>(reduction == 2 ? l / counted : l);
+        else sums[blockIdx.x] = make_double2(l, counted);
+    }
+}
+
+__global__ void __launch_bounds__(kThreads)
+loss_sum_kernel(const double2 *__restrict__ sums, int count, int reduction, float *__restrict__ loss) {
+    __shared__ double2 red[8];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    double l = 0.0, n = 0.0;
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const double2 x = sums[i];
+        l += x.x;
+        n += x.y;
+    }
+    l = warp_sum(l);
+    n = warp_sum(n);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_double2(l, n);
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 8; ++w) {
+        l += red[w].x;
+        n += red[w].y;
+    }
+    loss[0] = static_cast<float>(reduction == 2 ? l / n : l);
+}
+
+// Rows that count, of the whole batch (blocks that do not count for themselves wait for this).
+constexpr int kCountRows = 4096;
+__device__ int count_rows(const Targets &targets, int rows, int *red) {
+    int n = 0;
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) n += target_at(targets, i) >= 0;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) n += red[w];
+    return n;
+}
+__global__ void __launch_bounds__(1024)
+count_rows_kernel(Targets targets, int rows, int *count) {
+    __shared__ int red[32];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int n = count_rows(targets, rows, red);
+    if (threadIdx.x == 0) *count = n;
+}
+
+// Weights of the rows' losses in the result's gradient, g = grad, or grad / rows counted, 0 for rows left out; and a copy of x
+// whose rows are multiplied by them (scaled), or left out where they are zero.  A block takes rows in turn.
+__global__ void __launch_bounds__(kThreads)
+row_weights_kernel(const __grid_constant__ RowsIn x, Targets targets, int reduction, const float *__restrict__ grad, const int *count,
+                   float *__restrict__ weights, float *__restrict__ copy, int scaled) {
+    __shared__ int red[32];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    float all = 1.f;
+    if (reduction != 0) {
+        all = grad[0];
+        if (reduction == 2) all /= static_cast<float>(count ? *count : count_rows(targets, x.rows, red));
+    }
+    for (int row = blockIdx.x; row < x.rows; row += gridDim.x) {
+        const bool kept = target_at(targets, row) >= 0;
+        const float g = kept ? (reduction == 0 ? grad[row] : all) : 0.f;
+        if (threadIdx.x == 0) weights[row] = g;
+        if (!copy) continue;
+        const float *src = x.ptr + x.offset(row);
+        float *dst = copy + static_cast<long long>(row) * x.cols;
+        const float f = scaled ? g : 1.f;
+        for (int c = threadIdx.x; c < x.cols; c += kThreads) dst[c] = kept ? src[c * x.col_stride] * f : 0.f;
+    }
+}
+
+// z -> g * (exp(z - lse) - [j = t]), in place.
+__global__ void __launch_bounds__(kThreads)
+logit_grad_kernel(float *__restrict__ z, int n, FastDiv stretches, Targets targets, const float *__restrict__ lse,
+                  const float *__restrict__ weights) {
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int row = fd_div(blockIdx.x, stretches), c0 = static_cast<int>(blockIdx.x - row * stretches.d) * kStretch;
+    float *src = z + static_cast<long long>(row) * n;
+    const long long t = target_at(targets, row);
+    const float l = lse[row], g = weights[row];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c = c0 + i * kThreads + threadIdx.x;
+        if (c >= n) break;
+        float d = expf(src[c] - l) - (c == t ? 1.f : 0.f);
+        src[c] = t < 0 ? 0.f : t < n ? d * g : NAN;
+    }
+}
+
+}  // namespace
+
+int launch_logit_stats(const float *z, int64_t rows, int64_t n, const Targets &targets, float2 *pairs, float *at_target, cudaStream_t stream) {
+    const int64_t stretches = (n + kStretch - 1) / kStretch;
+    const dim3 grid(static_cast<unsigned>(rows * stretches));
+    const cudaError_t e = launch_dependent(logit_stats_kernel, grid, dim3(kThreads), 0, stream, z, static_cast<int>(rows), static_cast<int>(n),
+                                           make_fastdiv(stretches), targets, pairs, at_target);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "logit_stats_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("logit_stats_kernel");
+    return MNI_B200_OK;
+}
+
+size_t loss_sums_bytes(int64_t rows) { return static_cast<size_t>((rows + 31) / 32) * sizeof(double2); }
+
+int launch_loss_finish(const float2 *pairs, int64_t parts, int64_t rows, int64_t classes, const Targets &targets, const float *at_target,
+                       int reduction, float *loss, float *lse, double2 *sums, cudaStream_t stream) {
+    const unsigned blocks = static_cast<unsigned>((rows + 31) / 32);
+    cudaError_t e = launch_dependent(loss_finish_kernel, dim3(blocks), dim3(kThreads), 0, stream, pairs, static_cast<int>(parts),
+                                     static_cast<int>(rows), static_cast<int>(classes), targets, at_target, reduction, loss, lse, sums);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "loss_finish_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("loss_finish_kernel");
+    if (reduction == 0 || blocks == 1) return MNI_B200_OK;
+    e = launch_dependent(loss_sum_kernel, dim3(1), dim3(kThreads), 0, stream, sums, static_cast<int>(blocks), reduction, loss);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "loss_sum_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("loss_sum_kernel");
+    return MNI_B200_OK;
+}
+
+int launch_row_weights(const RowsIn &x, const Targets &targets, int reduction, const float *grad, int *count, float *weights, float *copy,
+                       bool scaled, int sm_count, cudaStream_t stream) {
+    const int *counted = nullptr;
+    if (reduction == 2 && x.rows > kCountRows) {
+        const cudaError_t e = launch_dependent(count_rows_kernel, dim3(1), dim3(1024), 0, stream, targets, x.rows, count);
+        if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "count_rows_kernel launch failed: %s", cudaGetErrorString(e));
+        MNI_LAUNCH_CHECK("count_rows_kernel");
+        counted = count;
+    }
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(x.rows, 8ll * sm_count));
+    const cudaError_t e = launch_dependent(row_weights_kernel, dim3(blocks), dim3(kThreads), 0, stream, x, targets, reduction, grad, counted,
+                                           weights, copy, scaled ? 1 : 0);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "row_weights_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("row_weights_kernel");
+    return MNI_B200_OK;
+}
+
+int launch_logit_grad(float *z, int64_t rows, int64_t n, const Targets &targets, const float *lse, const float *weights, cudaStream_t stream) {
+    const int64_t stretches = (n + kStretch - 1) / kStretch;
+    const dim3 grid(static_cast<unsigned>(rows * stretches));
+    const cudaError_t e = launch_dependent(logit_grad_kernel, grid, dim3(kThreads), 0, stream, z, static_cast<int>(n), make_fastdiv(stretches),
+                                           targets, lse, weights);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "logit_grad_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("logit_grad_kernel");
+    return MNI_B200_OK;
+}
+
+}  // namespace mni

@@ -1,0 +1,215 @@
+// Updates of matrices by their orthogonalised momentum: the kernels around the Newton-Schulz products.
+//
+//   m <- mu m + g;  u = g + mu m (nesterov), or m;  x0 = u / (|u|_F + eps)
+//   five times x <- a x + (b A + c A^2) x with A = x x^T (the other way round for matrices with more rows than columns)
+//   p <- decay p - scale x
+//
+// As in optimizer.cu the unit of work is a chunk of whichever matrix, and one launch covers a list of them.  Bound by memory: 12
+// bytes an element for the momentum (read g and m, write m), 8 to 12 for the normalised update, 12 for the parameter.  Norms are
+// summed in f64, in a fixed order.
+#include "internal.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mni {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxList = 256;                  // matrices per launch
+constexpr int kMaxChunks = 512;                // of one matrix: what a block adds up for the norm
+constexpr int kChunk = 4096;
+
+struct List {
+    float *param[kMaxList], *momentum[kMaxList], *x[kMaxList];
+    const float *grad[kMaxList];
+    long long n[kMaxList];
+    float scale[kMaxList];
+    unsigned first[kMaxList + 1];              // index of a matrix's first chunk
+    int chunk[kMaxList];                       // elements of one
+    int count;
+};
+
+__device__ __forceinline__ int find(const List &list, unsigned chunk) {
+    int lo = 0, hi = list.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (list.first[mid] <= chunk) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float update_of(float g, float m, float mu, bool nesterov) { return nesterov ? fmaf(mu, m, g) : m; }
+
+__global__ void __launch_bounds__(kThreads)
+muon_momentum_kernel(const __grid_constant__ List list, float mu, bool nesterov, double *__restrict__ partial) {
+    __shared__ double red[8];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int t = find(list, blockIdx.x);
+    const long long base = static_cast<long long>(blockIdx.x - list.first[t]) * list.chunk[t], end = min(list.n[t], base + list.chunk[t]);
+    float *const m = list.momentum[t];
+    const float *const g = list.grad[t];
+    double sum = 0.0;
+    auto one = [&](float gi, float &mi) {
+        float u = gi;
+        if (m) {
+            mi = fmaf(mu, mi, gi);
+            u = update_of(gi, mi, mu, nesterov);
+        }
+        sum += static_cast<double>(u) * u;
+    };
+    const bool vec = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+    long long i = base;
+    if (vec) {
+        for (; i + kThreads * 4 <= end; i += kThreads * 4) {
+            const long long at = i + threadIdx.x * 4;
+            const float4 gi = *reinterpret_cast<const float4 *>(g + at);
+            float4 mi = m ? *reinterpret_cast<const float4 *>(m + at) : gi;
+            one(gi.x, mi.x); one(gi.y, mi.y); one(gi.z, mi.z); one(gi.w, mi.w);
+            if (m) *reinterpret_cast<float4 *>(m + at) = mi;
+        }
+    }
+    for (i += threadIdx.x; i < end; i += kThreads) {
+        float mi = m ? m[i] : 0.f;
+        one(g[i], mi);
+        if (m) m[i] = mi;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) sum += red[w];
+        partial[blockIdx.x] = sum;
+    }
+}
+
+// 1 / (norm + eps) of matrix t, from its chunks' sums: the same in every block that asks.
+__device__ float inverse_norm(const List &list, int t, const double *partial, float eps, double *red) {
+    double sum = 0.0;
+    for (unsigned i = list.first[t] + threadIdx.x; i < list.first[t + 1]; i += kThreads) sum += __ldcg(partial + i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = red[0];
+    for (int w = 1; w < 8; ++w) sum += red[w];
+    return static_cast<float>(1.0 / (sqrt(sum) + static_cast<double>(eps)));
+}
+
+__global__ void __launch_bounds__(kThreads)
+muon_normalise_kernel(const __grid_constant__ List list, float mu, bool nesterov, float eps, const double *__restrict__ partial) {
+    __shared__ double red[8];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int t = find(list, blockIdx.x);
+    const float inverse = inverse_norm(list, t, partial, eps, red);
+    const long long base = static_cast<long long>(blockIdx.x - list.first[t]) * list.chunk[t], end = min(list.n[t], base + list.chunk[t]);
+    const float *const m = list.momentum[t], *const g = list.grad[t];
+    float *const x = list.x[t];
+    for (long long i = base + threadIdx.x; i < end; i += kThreads) x[i] = (m ? update_of(g[i], m[i], mu, nesterov) : g[i]) * inverse;
+}
+
+__global__ void __launch_bounds__(kThreads)
+muon_update_kernel(const __grid_constant__ List list, float decay) {
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int t = find(list, blockIdx.x);
+    const long long base = static_cast<long long>(blockIdx.x - list.first[t]) * list.chunk[t], end = min(list.n[t], base + list.chunk[t]);
+    float *const p = list.param[t];
+    const float *const x = list.x[t];
+    const float scale = list.scale[t];
+    for (long long i = base + threadIdx.x; i < end; i += kThreads) p[i] = fmaf(-scale, x[i], decay * p[i]);
+}
+
+__global__ void __launch_bounds__(kThreads)
+combine_kernel(const float *x, const float *y, float *out, long long n, float alpha, float beta) {
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads)
+        out[i] = fmaf(alpha, x[i], beta * y[i]);
+}
+
+int64_t chunk_of(int64_t n) {
+    const int64_t each = (n + kMaxChunks - 1) / kMaxChunks;
+    return std::max<int64_t>(kChunk, (each + kChunk - 1) / kChunk * kChunk);
+}
+int64_t chunks_of(int64_t n) { return (n + chunk_of(n) - 1) / chunk_of(n); }
+
+// Calls launch(list, chunks, chunks before) for stretches of the entries that fit a launch.
+template <class Launch>
+int for_lists(const MuonEntry *e, int64_t count, Launch launch) {
+    int64_t before = 0;
+    for (int64_t at = 0; at < count;) {
+        List list;
+        int64_t chunks = 0;
+        int k = 0;
+        for (; at < count && k < kMaxList; ++at) {
+            if (e[at].n == 0) continue;
+            list.param[k] = e[at].param;
+            list.momentum[k] = e[at].momentum;
+            list.x[k] = e[at].x;
+            list.grad[k] = e[at].grad;
+            list.n[k] = e[at].n;
+            list.scale[k] = e[at].scale;
+            list.chunk[k] = static_cast<int>(chunk_of(e[at].n));
+            list.first[k] = static_cast<unsigned>(chunks);
+            chunks += chunks_of(e[at].n);
+            ++k;
+        }
+        if (k == 0) break;
+        list.first[k] = static_cast<unsigned>(chunks);
+        list.count = k;
+        const int rc = launch(list, static_cast<unsigned>(chunks), before);
+        if (rc) return rc;
+        before += chunks;
+    }
+    return MNI_B200_OK;
+}
+
+}  // namespace
+
+size_t muon_partial_bytes(const MuonEntry *e, int64_t count) {
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < count; ++i) chunks += e[i].n ? chunks_of(e[i].n) : 0;
+    return static_cast<size_t>(chunks) * sizeof(double);
+}
+
+int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, cudaStream_t stream) {
+    int rc = for_lists(e, count, [&](const List &list, unsigned chunks, int64_t before) -> int {
+        const cudaError_t r = launch_dependent(muon_momentum_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, partial + before);
+        if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_momentum_kernel launch failed: %s", cudaGetErrorString(r));
+        MNI_LAUNCH_CHECK("muon_momentum_kernel");
+        return MNI_B200_OK;
+    });
+    if (rc) return rc;
+    return for_lists(e, count, [&](const List &list, unsigned chunks, int64_t before) -> int {
+        const cudaError_t r = launch_dependent(muon_normalise_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, eps,
+                                               static_cast<const double *>(partial + before));
+        if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_normalise_kernel launch failed: %s", cudaGetErrorString(r));
+        MNI_LAUNCH_CHECK("muon_normalise_kernel");
+        return MNI_B200_OK;
+    });
+}
+
+int launch_muon_update(const MuonEntry *e, int64_t count, float decay, cudaStream_t stream) {
+    return for_lists(e, count, [&](const List &list, unsigned chunks, int64_t) -> int {
+        const cudaError_t r = launch_dependent(muon_update_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, decay);
+        if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_update_kernel launch failed: %s", cudaGetErrorString(r));
+        MNI_LAUNCH_CHECK("muon_update_kernel");
+        return MNI_B200_OK;
+    });
+}
+
+int launch_combine(const float *x, const float *y, float *out, int64_t n, float alpha, float beta, cudaStream_t stream) {
+    if (n == 0) return MNI_B200_OK;
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((n + kThreads - 1) / kThreads, 8ll * device_sm_count()));
+    const cudaError_t e = launch_dependent(combine_kernel, dim3(blocks), dim3(kThreads), 0, stream, x, y, out, n, alpha, beta);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "combine_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("combine_kernel");
+    return MNI_B200_OK;
+}
+
+}  // namespace mni

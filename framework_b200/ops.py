@@ -128,6 +128,69 @@ def clip_and_step(params: Sequence[DeviceTensor], ms: Sequence[DeviceTensor], vs
     return float(np.sqrt(np.float32(sumsq.item())))
 
 
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _reduction(name: str) -> int:
+    if name not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, not {name!r}")
+    return _REDUCTIONS[name]
+
+
+def linear_cross_entropy(x: DeviceTensor, weight: DeviceTensor, targets: "torch.Tensor", bias: Optional[DeviceTensor] = None, *,
+                         reduction: str = "mean") -> Tuple[DeviceTensor, DeviceTensor]:
+    """Softmax cross entropy of ``x.weight (+ bias)`` without the logits in memory -> (loss, lse).
+
+    ``x`` is [.., K] (two dims at least), ``weight`` [K, N] with any strides (``permute`` of a stored [N, K] for a tied embedding), ``targets``
+    a torch tensor of int32 or int64 on x's device, of x's shape without the last dim.  A target below zero leaves its row out
+    (loss 0, no gradient); one of N or more makes its loss NaN.  ``reduction`` "none": losses of the rows' shape; "sum", "mean" (over the
+    rows that are not left out): one number, shape (1,).  ``lse``, the rows' log-sum-exp, is what the backward needs."""
+    return _host.linear_cross_entropy(x, weight, targets, bias, _reduction(reduction))
+
+
+def linear_cross_entropy_backward(grad: DeviceTensor, x: DeviceTensor, weight: DeviceTensor, targets: "torch.Tensor",
+                                  lse: DeviceTensor, bias: Optional[DeviceTensor] = None, *, reduction: str = "mean", flags: int = 0,
+                                  need_dx: bool = True, need_dw: bool = True, want_dbias: bool = False,
+                                  dx: Optional[DeviceTensor] = None, dw: Optional[DeviceTensor] = None,
+                                  dbias: Optional[DeviceTensor] = None):
+    """Backward of ``linear_cross_entropy`` -> (dx, dw[, dbias]); ``grad`` has the loss's shape.
+
+    ``dw`` has the weight's shape; it is laid out as the weight is stored, so the gradient of a transposing view of a stored [N, K] is such a
+    view itself.  With the ACCUMULATE flags the gradients are added to the ``dx``, ``dw``, ``dbias`` given."""
+    return _host.linear_cross_entropy_backward(grad, x, weight, targets, lse, bias, _reduction(reduction), flags, need_dx, need_dw,
+                                               want_dbias, dx, dw, dbias)
+
+
+# Coefficients of the Newton-Schulz step that Muon uses: five steps bring singular values from 1e-3 .. 1 to 0.7 .. 1.2.
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(g: DeviceTensor, *, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ,
+                  eps: float = 1e-7) -> DeviceTensor:
+    """Each matrix of g [.., rows, cols] divided by its Frobenius norm (+ eps), then ``steps`` times x <- a x + (b A + c A^2) x with
+    A = x x^T (from the right for more rows than columns): a matrix of the same singular vectors whose singular values are nearly one."""
+    a, b, c = coefficients
+    return _host.orthogonalize(g, int(steps), a, b, c, eps)
+
+
+def muon_step(params: Sequence[DeviceTensor], momenta: Sequence[DeviceTensor], grads: Sequence[DeviceTensor], *, lr: float,
+              momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+              coefficients: Sequence[float] = NEWTON_SCHULZ, eps: float = 1e-7, scale="shape") -> None:
+    """One step of Muon on a model's matrices (``clip_and_step`` is for the other parameters), in place:
+    m <- momentum m + grad; u = grad + momentum m (or m without ``nesterov``); p <- (1 - lr weight_decay) p - lr s orthogonalize(u).
+
+    Weights are [in, out], as ``Linear`` has them; leading dims count as that many matrices.  ``scale`` is s: "shape" for sqrt(max(1, out / in)),
+    "size" for 0.2 sqrt(max(in, out)), which gives updates the size of AdamW's, or a number."""
+    if isinstance(scale, str):
+        if scale not in ("shape", "size"):
+            raise ValueError(f"scale must be 'shape', 'size' or a number, not {scale!r}")
+        rule = 0 if scale == "shape" else 1
+    else:
+        rule = float(scale)
+    a, b, c = coefficients
+    _host.muon_step(params, momenta, grads, rule, lr, momentum, nesterov, weight_decay, int(steps), a, b, c, eps)
+
+
 def permute(a: DeviceTensor, dims: Sequence[int]) -> DeviceTensor:
     """``ops::layout::permute``: a stride-only view sharing the storage (what the reference's CPU backend
     does, ops/layout.rs:112-134); the matmul kernels read it in place."""

@@ -80,6 +80,7 @@ typedef enum mni_b200_status {
 #define MNI_B200_ACCUMULATE_DA      (1u << 2) /* bwd: da += ...                                             */
 #define MNI_B200_ACCUMULATE_DB      (1u << 3) /* bwd: db += ...                                             */
 #define MNI_B200_ACCUMULATE_DBIAS   (1u << 4) /* bwd: dbias += ...                                          */
+#define MNI_B200_DB_TRANSPOSED      (1u << 5) /* linear_cross_entropy_bwd: dw is laid out [N, K]                     */
 #define MNI_B200_FORCE_TENSOR_PATH  (1u << 8) /* tests: never take the skinny CUDA-core path                */
 #define MNI_B200_FORCE_SKINNY_PATH  (1u << 9) /* tests: take the skinny path whenever its kernel can run    */
 #define MNI_B200_FORCE_PACK         (1u << 10)/* tests: copy strided operands to scratch first              */
@@ -219,6 +220,56 @@ MNI_B200_API int mni_b200_clip_and_step(int64_t count, float *const *params, flo
                                         float *const *grads, const int64_t *n, float lr, float beta1, float beta2,
                                         float eps, float weight_decay, uint32_t step, float max_grad_norm, float *norm,
                                         void *stream);
+
+/*
+ * Softmax cross entropy of a projection: the loss of logits z = x.w (+ bias), x [.., K] with any leading dims (M rows in all), w
+ * [K, N], both with any strides, without the logits in memory of the caller's.  (The reference has the loss of logits that it
+ * is given, ops/loss.rs.)
+ *
+ *   lse[r] = log sum_j exp z[r, j]          loss[r] = lse[r] - z[r, targets[r]]
+ *
+ * `targets` are M whole numbers of `target_bytes` bytes (4 or 8).  One below zero leaves its row out: loss 0, no gradient,
+ * whatever its row of x holds.  One of N or more makes the row's loss NaN, and with it the gradients.
+ * `reduction`: NONE leaves M losses in `loss`; SUM and MEAN one number, MEAN over the rows that are not left out (NaN where there
+ * is none).  `lse` takes M numbers (those of rows left out too), which the backward needs.
+ */
+#define MNI_B200_REDUCE_NONE 0
+#define MNI_B200_REDUCE_SUM  1
+#define MNI_B200_REDUCE_MEAN 2
+MNI_B200_API int mni_b200_linear_cross_entropy_fwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias,
+                                                   const void *targets, int target_bytes, int reduction, float *loss,
+                                                   float *lse, uint32_t flags, void *stream);
+
+/*
+ * Its backward, from the forward's operands and `lse`.  `grad` is the gradient of `loss`: M numbers for NONE, else one.  dx takes x's
+ * shape and dw [K, N] (with MNI_B200_DB_TRANSPOSED laid out [N, K], for a weight stored so), contiguous; dbias N numbers.
+ * Each may be NULL.  The ACCUMULATE flags of mni_b200_matmul_bwd (DA: dx, DB: dw) add instead of overwriting.
+ */
+MNI_B200_API int mni_b200_linear_cross_entropy_bwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias,
+                                                   const void *targets, int target_bytes, int reduction, const float *lse,
+                                                   const float *grad, float *dx, float *dw, float *dbias, uint32_t flags,
+                                                   void *stream);
+
+/*
+ * Makes the singular values of matrices nearly one by `steps` Newton-Schulz steps: x = g / (|g|_F + eps), then
+ * x <- a x + (b A + c A^2) x with A = x x^T (from the right for matrices with more rows than columns).  g is [.., rows, cols] with any
+ * strides, each of its matrices by itself; `out` is contiguous in its shape and may be g's own memory where g is contiguous.
+ * (No counterpart in the reference.)
+ */
+MNI_B200_API int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float a, float b, float c, float eps,
+                                        void *stream);
+
+/*
+ * One step of Muon on a list of `count` contiguous matrices, beside mni_b200_clip_and_step for the other parameters:
+ *   momentum = mu * momentum + grad;  u = nesterov ? grad + mu * momentum : momentum
+ *   param = (1 - lr * weight_decay) * param - lr * scales[i] * orthogonalize(u)
+ * params and momenta are updated in place, grads are read; no two of an entry's three may share memory.  Entries that share memory with
+ * others are stepped one after the other, in list order.  (No counterpart in the reference.)
+ */
+MNI_B200_API int mni_b200_muon_step(int64_t count, float *const *params, float *const *momenta, const float *const *grads,
+                                    const int64_t *rows, const int64_t *cols, const float *scales, float lr, float momentum,
+                                    int nesterov, float weight_decay, int steps, float a, float b, float c, float eps,
+                                    void *stream);
 
 /*
  * Same result as mni_b200_add_bias_bwd, for callers that must never see this library
