@@ -1331,55 +1331,108 @@ RowsIn rows_in(const LossCall &l) {
     return r;
 }
 
-int loss_fwd_body(Call &c, const LossCall &l, float *loss, float *lse) {
-    if (l.M == 0) return MNI_B200_OK;
-    const int64_t stretches = (l.N + kLogitStretch - 1) / kLogitStretch;
-    if (l.M * stretches > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld classes are too many", (long long)l.M, (long long)l.N);
-    const size_t pairs = c.arena.reserve(static_cast<size_t>(stretches * l.M) * sizeof(float2));
-    const size_t picked = c.arena.reserve(static_cast<size_t>(l.M) * sizeof(float));
-    const size_t sums = c.arena.reserve(loss_sums_bytes(l.M));
-    mni_b200_view x;
-    int rc = rows_of_x(c, l, x);
+// Few rows, or few logits: products in f32 as the other entry points make them, logits in scratch.  Otherwise from 16-bit planes, logits
+// never in memory.
+constexpr int64_t kLossRows = 8;
+bool loss_from_planes(const LossCall &l) { return l.M > kLossRows && l.M * l.N * l.K > kTinyWork; }
+
+float *dry_pointer() { return reinterpret_cast<float *>(static_cast<uintptr_t>(256)); }
+
+// A view as 16-bit planes can be made of it: itself, or gathered.
+int for_planes(Call &c, const mni_b200_view *&v, mni_b200_view &packed) {
+    HalfView probe;
+    bool swapped;
+    if (view_to_half(*v, probe, &swapped)) return MNI_B200_OK;
+    const mni_b200_view **use[1] = {&v};
+    const int rc = pack_views(c, use, &packed, 1);
     if (rc) return rc;
-    const size_t z_at = c.arena.reserve(static_cast<size_t>(l.M * l.N) * sizeof(float));
-    float *const z = c.dry() ? reinterpret_cast<float *>(static_cast<uintptr_t>(256)) : c.at(z_at);
-    rc = fwd_body(c, &x, l.w, z, l.bias);
-    if (rc || c.dry()) return rc;
-    float2 *const p = reinterpret_cast<float2 *>(c.at(pairs));
-    rc = launch_logit_stats(z, l.M, l.N, l.targets, p, c.at(picked), c.stream);
-    if (rc) return rc;
-    return launch_loss_finish(p, stretches, l.M, l.N, l.targets, c.at(picked), l.reduction, loss, lse, reinterpret_cast<double2 *>(c.at(sums)),
-                              c.stream);
+    if (!view_to_half(*v, probe, &swapped)) return fail(MNI_B200_ERR_TOO_LARGE, "an operand exceeds the kernels' int32 indexing");
+    return MNI_B200_OK;
 }
 
-int loss_bwd_body(Call &c, const LossCall &l, const float *lse, const float *grad, float *dx, float *dw, float *dbias) {
-    if (!dx && !dw && !dbias) return MNI_B200_OK;
-    const bool turned = (c.flags & MNI_B200_DB_TRANSPOSED) != 0;
-    if (l.M == 0) {
-        int rc = dw ? zero_or_bias_fill(c, dw, l.K, l.N, nullptr, (c.flags & MNI_B200_ACCUMULATE_DB) != 0) : static_cast<int>(MNI_B200_OK);
-        if (rc == MNI_B200_OK && dbias) rc = zero_or_bias_fill(c, dbias, 1, l.N, nullptr, (c.flags & MNI_B200_ACCUMULATE_DBIAS) != 0);
-        return rc;
+// Longest contraction in one accumulator of the tensor core, whose adds truncate (7.5e-10 of the sum an element).
+constexpr int kLossChunkK = 1024;
+
+// z = x . w of the classes first .. first + count, from planes x (view `xi` of h) and w (view `wi`).
+GemmProblem logits_problem(const LossCall &l, const Halves &h, int wi, int64_t first, int64_t count, HalfOperand &x, HalfOperand &w) {
+    x = h.operand(0, false);
+    w = h.operand(wi, true);
+    w.ptr = static_cast<const uint16_t *>(w.ptr) + (w.k_major ? first * w.pitch : first);
+    w.rows = count;
+    GemmProblem p;
+    p.M = l.M; p.N = count; p.K = l.K;
+    p.ha = &x; p.hb = &w;
+    p.half_status = h.status + h.blocks;
+    p.chunk_k = kLossChunkK;
+    return p;
+}
+
+int loss_fwd_body(Call &c, const LossCall &l, float *loss, float *lse) {
+    if (l.M == 0) return MNI_B200_OK;
+    const bool planes = loss_from_planes(l);
+    const int64_t stretch = planes ? 128 : kLogitStretch, stretches = (l.N + stretch - 1) / stretch;
+    if (!planes && l.M * stretches > 0x7fffffffLL)
+        return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld classes are too many", (long long)l.M, (long long)l.N);
+    const size_t pairs_at = c.arena.reserve(static_cast<size_t>(stretches * l.M) * sizeof(float2));
+    const size_t picked_at = c.arena.reserve(static_cast<size_t>(l.M) * sizeof(float));
+    const size_t sums_at = c.arena.reserve(loss_sums_bytes(l.M));
+    float2 *const pairs = reinterpret_cast<float2 *>(c.dry() ? dry_pointer() : c.at(pairs_at));
+    float *const picked = c.dry() ? dry_pointer() : c.at(picked_at);
+    mni_b200_view x, packed[2];
+    int rc = rows_of_x(c, l, x);
+    if (rc) return rc;
+    if (planes) {
+        const mni_b200_view *xv = &x, *wv = l.w;
+        rc = for_planes(c, xv, packed[0]);
+        if (rc == MNI_B200_OK) rc = for_planes(c, wv, packed[1]);
+        if (rc) return rc;
+        Halves h;
+        rc = make_halves(c, {xv, wv}, h);
+        c.used_half = false;                       // there is no other way to go on without the scratch
+        if (rc || c.dry()) return rc;
+        HalfOperand xo, wo;
+        const GemmProblem p = logits_problem(l, h, 1, 0, l.N, xo, wo);
+        FusedArgs f{};
+        f.targets = l.targets;
+        f.classes = static_cast<int>(l.N);
+        f.bias = l.bias;
+        f.pairs = pairs;
+        f.at_target = picked;
+        rc = launch_gemm_fused(p, kFusedPairs, f, false, c.st->err_word, c.gemm_sms(), c.stream);
+    } else {
+        const size_t z_at = c.arena.reserve(static_cast<size_t>(l.M * l.N) * sizeof(float));
+        float *const z = c.dry() ? dry_pointer() : c.at(z_at);
+        rc = fwd_body(c, &x, l.w, z, l.bias);
+        if (rc || c.dry()) return rc;
+        rc = launch_logit_stats(z, l.M, l.N, l.targets, pairs, picked, c.stream);
     }
+    if (rc) return rc;
+    return launch_loss_finish(pairs, stretches, l.M, l.N, l.targets, picked, l.reduction, loss, lse,
+                              reinterpret_cast<double2 *>(c.at(sums_at)), c.stream);
+}
+
+// The backward with logits in scratch.
+int loss_bwd_small(Call &c, const LossCall &l, const float *lse, const float *grad, float *dx, float *dw, float *dbias) {
+    const bool turned = (c.flags & MNI_B200_DB_TRANSPOSED) != 0;
     const int64_t stretches = (l.N + kLogitStretch - 1) / kLogitStretch;
     if (l.M * stretches > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld classes are too many", (long long)l.M, (long long)l.N);
     const size_t count = c.arena.reserve(sizeof(int));
     const size_t weights = c.arena.reserve(static_cast<size_t>(l.M) * sizeof(float));
     const size_t copy = c.arena.reserve(static_cast<size_t>(l.M * l.K) * sizeof(float));
-    float *const fake = reinterpret_cast<float *>(static_cast<uintptr_t>(256));
     mni_b200_view x{};
-    x.ptr = c.dry() ? fake : c.at(copy);
+    x.ptr = c.dry() ? dry_pointer() : c.at(copy);
     x.ndim = 2;
     x.shape[0] = l.M; x.shape[1] = l.K;
     x.stride[0] = l.K; x.stride[1] = 1;
     int rc = MNI_B200_OK;
     if (!c.dry()) {
         rc = launch_row_weights(rows_in(l), l.targets, l.reduction, grad, reinterpret_cast<int *>(c.at(count)), c.at(weights), c.at(copy), false,
-                                c.st->sm_count, c.stream);
+                                nullptr, c.st->sm_count, c.stream);
         if (rc) return rc;
     }
     const size_t z_at = c.arena.reserve(static_cast<size_t>(l.M * l.N) * sizeof(float));
     mni_b200_view z{};
-    z.ptr = c.dry() ? fake : c.at(z_at);
+    z.ptr = c.dry() ? dry_pointer() : c.at(z_at);
     z.ndim = 2;
     z.shape[0] = l.M; z.shape[1] = l.N;
     z.stride[0] = l.N; z.stride[1] = 1;
@@ -1403,63 +1456,296 @@ int loss_bwd_body(Call &c, const LossCall &l, const float *lse, const float *gra
     return rc;
 }
 
-// ------------------------------------------------------------------ Newton-Schulz updates
-struct MuonMatrix {
-    int64_t rows, cols, index;     // index: of its entry
-};
-struct NewtonSchulz {
-    int steps;
-    float a, b, c;
-};
+// Classes of a piece of the backward: a multiple of 256.
+constexpr int64_t kPieceBytes = 384ll << 20;
+int64_t piece_of(const LossCall &l) {
+    const int64_t fits = std::max<int64_t>(256, kPieceBytes / (6 * l.M) / 256 * 256);
+    const int env = env_int("MNI_B200_LOSS_PIECE", 0);
+    return std::min<int64_t>((l.N + 255) / 256 * 256, env > 0 ? (env + 255) / 256 * 256 : fits);
+}
 
-// The steps on `e`'s normalised updates, in place (e[i].x), one matrix after the other.
-int newton_schulz(Call &c, const NewtonSchulz &ns, const MuonMatrix &m, float *x) {
-    const bool tall = m.rows > m.cols;
-    const int64_t side = std::min(m.rows, m.cols), n = m.rows * m.cols;
-    const size_t mark = c.arena.used;
-    const size_t a_at = c.arena.reserve(static_cast<size_t>(side * side) * 4), q_at = c.arena.reserve(static_cast<size_t>(side * side) * 4),
-                 y_at = c.arena.reserve(static_cast<size_t>(n) * 4);
-    float *const fake = reinterpret_cast<float *>(static_cast<uintptr_t>(256));
-    float *const a = c.dry() ? fake : c.at(a_at), *const q = c.dry() ? fake : c.at(q_at), *const y = c.dry() ? fake : c.at(y_at);
-    auto view = [](float *p, int64_t r, int64_t k, bool turned) {
-        mni_b200_view v{};
-        v.ptr = p;
-        v.ndim = 2;
-        v.shape[0] = turned ? k : r; v.shape[1] = turned ? r : k;
-        v.stride[0] = turned ? 1 : k; v.stride[1] = turned ? k : 1;
-        return v;
-    };
-    const mni_b200_view X = view(x, m.rows, m.cols, false), XT = view(x, m.rows, m.cols, true), A = view(a, side, side, false), Q = view(q, side, side, false);
-    int rc = MNI_B200_OK;
-    const size_t inner = c.arena.used;
-    for (int s = 0; s < ns.steps && rc == MNI_B200_OK; ++s) {
-        c.arena.used = inner;
-        rc = tall ? fwd_body(c, &XT, &X, a, nullptr) : fwd_body(c, &X, &XT, a, nullptr);
-        if (rc == MNI_B200_OK) rc = fwd_body(c, &A, &A, q, nullptr);
-        if (rc == MNI_B200_OK && !c.dry()) rc = launch_combine(a, q, q, side * side, ns.b, ns.c, c.stream);
-        if (rc == MNI_B200_OK) rc = tall ? fwd_body(c, &X, &Q, y, nullptr) : fwd_body(c, &Q, &X, y, nullptr);
-        if (rc == MNI_B200_OK && !c.dry()) rc = launch_combine(x, y, x, n, ns.a, 1.f, c.stream);
-        if (c.dry()) break;
+// The backward from 16-bit planes: of one piece of the classes after the other the logits' gradients d, as planes, and both products with
+// them.  d carries no weights of rows, so that its range is known: w goes into the copy of x that dw is made of, and into dx at the
+// end.
+int loss_bwd_planes(Call &c, const LossCall &l, const float *lse, const float *grad, float *dx, float *dw, float *dbias) {
+    const bool turned = (c.flags & MNI_B200_DB_TRANSPOSED) != 0;
+    const uint32_t flags = c.flags;
+    struct Restore {
+        Call &c;
+        uint32_t flags;
+        ~Restore() { c.flags = flags; }
+    } restore{c, flags};
+    c.flags = 0;
+    const size_t words = c.arena.reserve(2 * sizeof(int));
+    const size_t weights_at = c.arena.reserve(static_cast<size_t>(l.M) * sizeof(float));
+    const size_t copy = dw ? c.arena.reserve(static_cast<size_t>(l.M * l.K) * sizeof(float)) : 0;
+    const int64_t sum_ld = round_up(l.K, 4);
+    const size_t sum_at = dx ? c.arena.reserve(static_cast<size_t>(l.M * sum_ld) * sizeof(float)) : 0;
+    float *const weights = c.dry() ? dry_pointer() : c.at(weights_at), *const sum = c.dry() ? dry_pointer() : c.at(sum_at);
+    int *const exponent = reinterpret_cast<int *>(c.dry() ? dry_pointer() : c.at(words)) + 1;
+    mni_b200_view x, weighted{}, packed[2];
+    int rc = rows_of_x(c, l, x);
+    if (rc) return rc;
+    const mni_b200_view *xv = &x, *wv = l.w;
+    rc = for_planes(c, xv, packed[0]);
+    if (rc == MNI_B200_OK) rc = for_planes(c, wv, packed[1]);
+    if (rc) return rc;
+    if (!c.dry()) {
+        rc = launch_row_weights(rows_in(l), l.targets, l.reduction, grad, exponent - 1, weights, dw ? c.at(copy) : nullptr, true, exponent,
+                                c.st->sm_count, c.stream);
+        if (rc) return rc;
     }
-    c.arena.used = mark;
+    weighted.ptr = c.dry() ? dry_pointer() : c.at(copy);
+    weighted.ndim = 2;
+    weighted.shape[0] = l.M; weighted.shape[1] = l.K;
+    weighted.stride[0] = l.K; weighted.stride[1] = 1;
+    Halves h;
+    rc = dw ? make_halves(c, {xv, wv, &weighted}, h) : make_halves(c, {xv, wv}, h);
+    c.used_half = false;
+    if (rc) return rc;
+    const int64_t piece = piece_of(l), plane = l.M * piece;
+    const size_t d_at = c.arena.reserve(static_cast<size_t>(plane) * 3 * 2);
+    const size_t mark = c.arena.used;
+    for (int64_t first = 0; first < l.N; first += piece) {
+        c.arena.used = mark;
+        const int64_t count = std::min(piece, l.N - first);
+        HalfOperand xo, wo;
+        HalfOperand d;
+        d.ptr = c.dry() ? dry_pointer() : c.at(d_at);
+        d.pitch = round_up(count, 64);
+        d.matrix = d.plane = l.M * d.pitch;
+        d.exp = exponent;
+        if (!c.dry()) {
+            const GemmProblem z = logits_problem(l, h, 1, first, count, xo, wo);
+            FusedArgs f{};
+            f.targets = l.targets;
+            f.first_class = static_cast<int>(first);
+            f.classes = static_cast<int>(l.N);
+            f.bias = l.bias;
+            f.lse = lse;
+            f.dst = static_cast<uint16_t *>(const_cast<void *>(d.ptr));
+            f.dst_pitch = d.pitch;
+            f.dst_plane = d.plane;
+            rc = launch_gemm_fused(z, kFusedGrads, f, false, c.st->err_word, c.gemm_sms(), c.stream);
+            if (rc) return rc;
+        }
+        GemmProblem p[2];
+        HalfOperand a[2], b[2];
+        int n = 0;
+        if (dx) {
+            a[n] = d;
+            a[n].k_major = true;
+            a[n].rows = l.M;
+            a[n].kdim = count;
+            b[n] = h.operand(1, false);
+            b[n].ptr = static_cast<const uint16_t *>(b[n].ptr) + (b[n].k_major ? first : first * b[n].pitch);
+            b[n].kdim = count;
+            p[n].M = l.M; p[n].N = l.K; p[n].K = count;
+            p[n].C = sum;
+            p[n].ldc = sum_ld;
+            p[n].accumulate = first > 0;
+            ++n;
+        }
+        if (dw) {
+            HalfOperand &of_x = turned ? b[n] : a[n], &of_d = turned ? a[n] : b[n];
+            of_x = h.operand(2, true);
+            of_d = d;
+            of_d.k_major = false;
+            of_d.rows = count;
+            of_d.kdim = l.M;
+            p[n].M = turned ? count : l.K; p[n].N = turned ? l.K : count; p[n].K = l.M;
+            p[n].C = dw + (turned ? first * l.K : first);
+            p[n].ldc = turned ? l.K : l.N;
+            p[n].accumulate = (flags & MNI_B200_ACCUMULATE_DB) != 0;
+            ++n;
+        }
+        for (int i = 0; i < n; ++i) p[i].chunk_k = kLossChunkK;
+        if (n) rc = run_halves(c, p, n, h, a, b, nullptr);
+        if (rc == MNI_B200_OK && dbias) {
+            const size_t part = c.arena.reserve(grad_column_sums_bytes(l.M, count, c.st->sm_count));
+            if (!c.dry())
+                rc = launch_grad_column_sums(static_cast<const uint16_t *>(d.ptr), d.pitch, d.plane, l.M, count, weights, h.status + h.blocks,
+                                             c.at(part), dbias + first, (flags & MNI_B200_ACCUMULATE_DBIAS) != 0, c.st->sm_count, c.stream);
+        }
+        if (rc) return rc;
+    }
+    if (dx && !c.dry())
+        rc = launch_scale_rows(sum, sum_ld, weights, dx, l.M, l.K, (flags & MNI_B200_ACCUMULATE_DA) != 0, c.st->sm_count, c.stream);
     return rc;
 }
 
-int muon_body(Call &c, std::vector<MuonEntry> &e, const std::vector<MuonMatrix> &shapes, const NewtonSchulz &ns, float mu, bool nesterov, float eps,
-              float decay, bool scratch_x) {
-    const int64_t count = static_cast<int64_t>(e.size());
-    const size_t partial = c.arena.reserve(muon_partial_bytes(e.data(), count));
-    if (scratch_x)
-        for (MuonEntry &m : e) {
-            const size_t at = c.arena.reserve(static_cast<size_t>(m.n) * sizeof(float));
-            m.x = c.dry() ? reinterpret_cast<float *>(static_cast<uintptr_t>(256)) : c.at(at);
+int loss_bwd_body(Call &c, const LossCall &l, const float *lse, const float *grad, float *dx, float *dw, float *dbias) {
+    if (!dx && !dw && !dbias) return MNI_B200_OK;
+    if (l.M == 0) {
+        int rc = dw ? zero_or_bias_fill(c, dw, l.K, l.N, nullptr, (c.flags & MNI_B200_ACCUMULATE_DB) != 0) : static_cast<int>(MNI_B200_OK);
+        if (rc == MNI_B200_OK && dbias) rc = zero_or_bias_fill(c, dbias, 1, l.N, nullptr, (c.flags & MNI_B200_ACCUMULATE_DBIAS) != 0);
+        return rc;
+    }
+    return loss_from_planes(l) ? loss_bwd_planes(c, l, lse, grad, dx, dw, dbias) : loss_bwd_small(c, l, lse, grad, dx, dw, dbias);
+}
+
+// ------------------------------------------------------------------ Newton-Schulz updates
+struct NewtonSchulz {
+    int steps;
+    double a, b, c;
+};
+
+// What the matrices of a step can hold at most, so that their planes' exponents need no pass over the data: singular values s of x
+// lie in [0, top] at first 1, A = x x^T holds s^2, Q = b A + c A^2 holds b t + c t^2 of t = s^2, the next x holds s (a + b t + c t^2).
+// No element of a matrix is larger than its largest singular value.
+struct StepScales {
+    int x, a, q;                   // exponents of the planes of x, A, Q
+};
+int step_scales(const NewtonSchulz &ns, std::vector<StepScales> &out) {
+    constexpr double kRounding = 1.01;
+    auto exponent = [](double bound) { return bound > 0 ? std::max(-40, std::min(40, 15 - static_cast<int>(std::ceil(std::log2(bound))))) : 0; };
+    double top = kRounding;
+    for (int k = 0; k < ns.steps; ++k) {
+        const double t = top * top;
+        auto q = [&](double y) { return std::fabs(ns.b * y + ns.c * y * y); };
+        double most_q = std::max(q(t), 1e-30);
+        if (ns.c != 0 && -ns.b / (2 * ns.c) > 0 && -ns.b / (2 * ns.c) < t) most_q = std::max(most_q, q(-ns.b / (2 * ns.c)));
+        auto p = [&](double y) { return std::sqrt(y) * std::fabs(ns.a + ns.b * y + ns.c * y * y); };
+        double most_p = p(t);
+        // inner extrema: 5 c y^2 + 3 b y + a = 0
+        const double qa = 5 * ns.c, qb = 3 * ns.b, disc = qb * qb - 4 * qa * ns.a;
+        if (qa == 0) {
+            if (qb != 0 && -ns.a / qb > 0 && -ns.a / qb < t) most_p = std::max(most_p, p(-ns.a / qb));
+        } else if (disc >= 0) {
+            for (const double sign : {-1.0, 1.0}) {
+                const double y = (-qb + sign * std::sqrt(disc)) / (2 * qa);
+                if (y > 0 && y < t) most_p = std::max(most_p, p(y));
+            }
         }
-    int rc = MNI_B200_OK;
-    if (!c.dry()) rc = launch_muon_start(e.data(), count, mu, nesterov, eps, reinterpret_cast<double *>(c.at(partial)), c.stream);
-    for (int64_t i = 0; i < count && rc == MNI_B200_OK; ++i)
-        if (e[i].n) rc = newton_schulz(c, ns, shapes[i], e[i].x);
-    if (rc == MNI_B200_OK && !c.dry() && scratch_x) rc = launch_muon_update(e.data(), count, decay, c.stream);
-    return rc;
+        out.push_back(StepScales{exponent(top), exponent(t), exponent(most_q)});
+        top = kRounding * std::max(most_p, 1e-30);
+        if (!(top < 1e9) || !(most_q < 1e9))
+            return fail(MNI_B200_ERR_ARG, "with these coefficients step %d can make singular values larger than 1e9", k + 1);
+    }
+    return MNI_B200_OK;
+}
+
+// Steps on `count` matrices of one shape, from planes (x[0] holds the start) to f32 `out` [count][rows][cols].
+struct MuonGroup {
+    int64_t rows, cols, side, count;
+    int64_t x_pitch, x_matrix, s_pitch, s_matrix;          // of x, and of A and Q
+    MuonGroup(int64_t r, int64_t c, int64_t n)
+        : rows(r), cols(c), side(std::min(r, c)), count(n), x_pitch(round_up(c, 64)), x_matrix(r * x_pitch), s_pitch(round_up(side, 64)),
+          s_matrix(side * s_pitch) {}
+    size_t x_bytes() const { return static_cast<size_t>(count * x_matrix) * 4; }
+    size_t s_bytes() const { return static_cast<size_t>(count * s_matrix) * 4; }
+};
+int newton_schulz(Call &c, const NewtonSchulz &ns, const std::vector<StepScales> &scales, const MuonGroup &g, uint16_t *const (&x)[2], uint16_t *a,
+                  uint16_t *q, float *out) {
+    const bool tall = g.rows > g.cols;
+    auto operand = [&](const uint16_t *p, bool of_x, bool k_major) {
+        HalfOperand o;
+        o.ptr = p;
+        o.k_major = k_major;
+        const int64_t rows = of_x ? g.rows : g.side, cols = of_x ? g.cols : g.side;
+        o.rows = k_major ? rows : cols;
+        o.kdim = k_major ? cols : rows;
+        o.pitch = of_x ? g.x_pitch : g.s_pitch;
+        o.matrix = of_x ? g.x_matrix : g.s_matrix;
+        o.plane = o.matrix * g.count;
+        o.batch = g.count;
+        o.planes = 2;
+        return o;
+    };
+    auto product = [&](const HalfOperand &l, const HalfOperand &r, const uint16_t *add, bool add_x, double alpha, double beta, uint16_t *dst, bool dst_x,
+                       float *final_out) {
+        GemmProblem p;
+        p.M = l.rows; p.N = r.rows; p.K = l.kdim;
+        p.batch = g.count;
+        p.ha = &l; p.hb = &r;
+        p.chunk_k = kLossChunkK;
+        FusedArgs f{};
+        f.alpha = static_cast<float>(alpha);
+        f.beta = static_cast<float>(beta);
+        f.add = add;
+        f.add_pitch = add_x ? g.x_pitch : g.s_pitch;
+        f.add_matrix = add_x ? g.x_matrix : g.s_matrix;
+        f.add_plane = f.add_matrix * g.count;
+        f.dst = dst;
+        f.dst_pitch = dst_x ? g.x_pitch : g.s_pitch;
+        f.dst_matrix = dst_x ? g.x_matrix : g.s_matrix;
+        f.dst_plane = f.dst_matrix * g.count;
+        if (final_out) {
+            f.final = 1;
+            p.C = final_out;
+            p.ldc = g.cols;
+            p.c_bstride = g.rows * g.cols;
+        }
+        f.mirror = dst_x ? 0 : 1;
+        return launch_gemm_fused(p, kFusedPolynomial, f, !dst_x, c.st->err_word, c.gemm_sms(), c.stream);
+    };
+    for (int k = 0; k < ns.steps; ++k) {
+        const StepScales &e = scales[static_cast<size_t>(k)];
+        const bool last = k + 1 == ns.steps;
+        const int next = last ? 0 : scales[static_cast<size_t>(k) + 1].x;
+        uint16_t *const from = x[k & 1], *const to = x[(k + 1) & 1];
+        // A = x x^T, or x^T x; the operands are the same planes
+        const HalfOperand xs = operand(from, true, !tall), as = operand(a, false, true), qs = operand(q, false, true);
+        int rc = product(xs, xs, nullptr, false, std::ldexp(1.0, e.a - 2 * e.x), 0.0, a, false, nullptr);
+        if (rc == MNI_B200_OK) rc = product(as, as, a, false, std::ldexp(ns.c, e.q - 2 * e.a), std::ldexp(ns.b, e.q - e.a), q, false, nullptr);
+        if (rc) return rc;
+        const double alpha = std::ldexp(1.0, next - e.q - e.x), beta = std::ldexp(ns.a, next - e.x);
+        if (tall) rc = product(operand(from, true, true), qs, from, true, alpha, beta, to, true, last ? out : nullptr);      // x Q
+        else rc = product(qs, operand(from, true, false), from, true, alpha, beta, to, true, last ? out : nullptr);          // Q x
+        if (rc) return rc;
+    }
+    return MNI_B200_OK;
+}
+
+// Scratch that the matrices which are worked on at a time may take: enough to fill the GPU many times over.
+constexpr size_t kMuonScratch = size_t{1} << 30;
+
+// The entries are `e`; where an entry has a parameter it is updated, otherwise the result goes to e[i].x (matrix after matrix).
+int muon_body(Call &c, const std::vector<MuonEntry> &e, const NewtonSchulz &ns, const std::vector<StepScales> &scales, float mu, bool nesterov, float eps,
+              float decay) {
+    // matrices of one shape, in the order of their first
+    std::map<std::pair<int64_t, int64_t>, size_t> index;
+    std::vector<std::vector<MuonEntry>> groups;
+    for (const MuonEntry &m : e) {
+        const auto found = index.emplace(std::make_pair(m.rows, m.cols), groups.size());
+        if (found.second) groups.emplace_back();
+        groups[found.first->second].push_back(m);
+    }
+    for (std::vector<MuonEntry> &all : groups) {
+        const MuonGroup one(all[0].rows, all[0].cols, 1);
+        const bool update = all[0].param != nullptr;
+        if (one.x_matrix / 8 > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "a matrix of %lld x %lld is too large", (long long)one.rows, (long long)one.cols);
+        const size_t each = 2 * one.x_bytes() + 2 * one.s_bytes() + (update ? static_cast<size_t>(one.rows * one.cols) * 4 : 0);
+        const int64_t at_once = std::max<int64_t>(1, std::min<int64_t>(65535, static_cast<int64_t>(kMuonScratch / each)));
+        for (size_t first = 0; first < all.size(); first += static_cast<size_t>(at_once)) {
+            const int64_t count = std::min<int64_t>(at_once, static_cast<int64_t>(all.size() - first));
+            MuonEntry *const part = all.data() + first;
+            const MuonGroup g(one.rows, one.cols, count);
+            const size_t mark = c.arena.used;
+            const size_t sums = c.arena.reserve(muon_partial_bytes(part, count)), x0 = c.arena.reserve(g.x_bytes()), x1 = c.arena.reserve(g.x_bytes()),
+                         a = c.arena.reserve(g.s_bytes()), q = c.arena.reserve(g.s_bytes()),
+                         result = update ? c.arena.reserve(static_cast<size_t>(count * g.rows * g.cols) * 4) : 0;
+            c.arena.used = mark;
+            if (c.dry()) continue;
+            if (update)
+                for (int64_t i = 0; i < count; ++i) part[i].x = c.at(result) + i * g.rows * g.cols;
+            MuonPlanes planes;
+            if (ns.steps > 0) {
+                planes.dst = reinterpret_cast<uint16_t *>(c.at(x0));
+                planes.pitch = g.x_pitch;
+                planes.matrix = g.x_matrix;
+                planes.plane = g.x_matrix * count;
+                planes.exponent = scales[0].x;
+            }
+            int rc = launch_muon_start(part, count, mu, nesterov, eps, reinterpret_cast<double *>(c.at(sums)), planes, c.stream);
+            uint16_t *const x[2] = {reinterpret_cast<uint16_t *>(c.at(x0)), reinterpret_cast<uint16_t *>(c.at(x1))};
+            if (rc == MNI_B200_OK)
+                rc = newton_schulz(c, ns, scales, g, x, reinterpret_cast<uint16_t *>(c.at(a)), reinterpret_cast<uint16_t *>(c.at(q)), part[0].x);
+            if (rc == MNI_B200_OK && update) rc = launch_muon_update(part, count, decay, c.stream);
+            if (rc) return rc;
+        }
+    }
+    return MNI_B200_OK;
 }
 
 // Stretches of memory, to find whether any is touched twice.
@@ -1491,12 +1777,12 @@ bool share_memory(const float *p, const float *q, int64_t n) {
     return a.first < b.second && b.first < a.second;
 }
 
-int check_newton_schulz(int steps, float a, float b, float c, float eps, NewtonSchulz &ns) {
+int check_newton_schulz(int steps, float a, float b, float c, float eps, NewtonSchulz &ns, std::vector<StepScales> &scales) {
     if (steps < 0 || steps > 100) return fail(MNI_B200_ERR_ARG, "%d steps", steps);
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return fail(MNI_B200_ERR_ARG, "coefficients must be finite");
     if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(MNI_B200_ERR_ARG, "eps must be zero or more");
     ns = NewtonSchulz{steps, a, b, c};
-    return MNI_B200_OK;
+    return step_scales(ns, scales);
 }
 int check_matrix(int64_t rows, int64_t cols) {
     if (rows < 0 || cols < 0) return fail(MNI_B200_ERR_ARG, "negative extent");
@@ -1850,7 +2136,8 @@ int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float 
     int rc = check_view(g, "g", 2);
     if (rc) return rc;
     NewtonSchulz ns;
-    rc = check_newton_schulz(steps, a, b, c, eps, ns);
+    std::vector<StepScales> scales;
+    rc = check_newton_schulz(steps, a, b, c, eps, ns, scales);
     if (rc) return rc;
     const int64_t rows = g->shape[g->ndim - 2], cols = g->shape[g->ndim - 1], batch = prod(g->shape, g->ndim - 2);
     rc = check_matrix(rows, cols);
@@ -1875,12 +2162,9 @@ int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float 
             src = out;
         }
         std::vector<MuonEntry> e;
-        std::vector<MuonMatrix> shapes;
-        for (int64_t i = 0; i < batch; ++i) {
-            e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, rows * cols, 0.f});
-            shapes.push_back(MuonMatrix{rows, cols, i});
-        }
-        return muon_body(call, e, shapes, ns, 0.f, false, eps, 1.f, false);
+        for (int64_t i = 0; i < batch; ++i)
+            e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, rows, cols, rows * cols, 0.f});
+        return muon_body(call, e, ns, scales, 0.f, false, eps, 1.f);
     });
 }
 
@@ -1890,10 +2174,10 @@ int mni_b200_muon_step(int64_t count, float *const *params, float *const *moment
     if (count < 0) return fail(MNI_B200_ERR_ARG, "negative count");
     if (count > 0 && (!params || !momenta || !grads || !rows || !cols || !scales)) return fail(MNI_B200_ERR_ARG, "null pointer");
     NewtonSchulz ns;
-    int rc = check_newton_schulz(steps, a, b, c, eps, ns);
+    std::vector<StepScales> bounds;
+    int rc = check_newton_schulz(steps, a, b, c, eps, ns, bounds);
     if (rc) return rc;
     std::vector<MuonEntry> e;
-    std::vector<MuonMatrix> shapes;
     for (int64_t i = 0; i < count; ++i) {
         rc = check_matrix(rows[i], cols[i]);
         if (rc) return rc;
@@ -1902,8 +2186,7 @@ int mni_b200_muon_step(int64_t count, float *const *params, float *const *moment
         if (!params[i] || !momenta[i] || !grads[i]) return fail(MNI_B200_ERR_ARG, "null pointer");
         if (share_memory(params[i], momenta[i], n) || share_memory(params[i], grads[i], n) || share_memory(momenta[i], grads[i], n))
             return fail(MNI_B200_ERR_ARG, "entry %lld: param, momentum and grad share memory", (long long)i);
-        e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, n, lr * scales[i]});
-        shapes.push_back(MuonMatrix{rows[i], cols[i], i});
+        e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, rows[i], cols[i], n, lr * scales[i]});
     }
     // Entries that share memory with one before them begin another round, which starts from what that one left.
     for (size_t first = 0; first < e.size();) {
@@ -1918,11 +2201,9 @@ int mni_b200_muon_step(int64_t count, float *const *params, float *const *moment
             written.add(m.momentum, m.n);
             read.add(m.grad, m.n);
         }
-        std::vector<MuonEntry> round(e.begin() + first, e.begin() + end);
-        const std::vector<MuonMatrix> sizes(shapes.begin() + first, shapes.begin() + end);
-        rc = with_scratch(0, stream, [&](Call &call) -> int {
-            return muon_body(call, round, sizes, ns, momentum, nesterov != 0, eps, 1.f - lr * weight_decay, true);
-        });
+        const std::vector<MuonEntry> round(e.begin() + first, e.begin() + end);
+        rc = with_scratch(0, stream,
+                          [&](Call &call) { return muon_body(call, round, ns, bounds, momentum, nesterov != 0, eps, 1.f - lr * weight_decay); });
         if (rc) return rc;
         first = end;
     }

@@ -40,6 +40,9 @@
 //               16 elements), 1.8 -> 0.96 ms.
 // Operands whose range f16 does not hold come as three (two) bf16 planes through the same stages.
 //
+// Three epilogues of kHalfThree keep a product out of memory altogether (fused_epilogue.h): the pairs (maximum, sum of exponentials) of
+// logits, the gradient of logits as planes for the products that follow, and a polynomial in a matrix, planes again.
+//
 // CG = 2: two CTAs of a cluster share a 256 x BN tile (cta_group::2 MMAs issued by the leader).
 // Work is dealt out as whole tiles, round-robin over the CTAs (pairs).  The tiles of a badly ragged wave are cut into
 // several units each, whose partial tiles go to scratch and are added by tail_finish_kernel (cut_tail has the rule).  On
@@ -56,6 +59,7 @@
 // test shortens it) the waiter records a code in a global error word, raises a CTA-wide abort flag and
 // all roles drain to the common exit, where TMEM is released.  Nothing traps.
 #include "activation.h"
+#include "fused_epilogue.h"
 #include "internal.h"
 
 #include <stdio.h>
@@ -80,7 +84,9 @@ constexpr int kBarBytes = (3 * kMaxStages + 4) * 8 + 16;
 constexpr long long kWaitCycles = 4000000000LL;            // default limit of every device-side wait: ~2 s at 2 GHz
 
 enum OperandMode { kKMajor = 0, kMnMultiBox = 1, kMnSingleBox = 2 };
-enum TailMode { kWholeTiles = 0, kBalanced = 1, kCutTiles = 2, kRunningSum = 3 };
+enum TailMode { kWholeTiles = 0, kBalanced = 1, kCutTiles = 2, kRunningSum = 3, kRowStats = 4, kRowGrads = 5, kPolynomial = 6 };
+// The last three: whole tiles of kHalfThree with an epilogue of their own.
+__host__ __device__ constexpr bool is_fused(int tail) { return tail >= kRowStats; }
 // How a product is computed: operands as f32 (three TF32 passes, or one), or as the 16-bit halves that split_half_kernel has made
 // of them (three passes, or one).
 enum PassMode { kThreePass = 0, kOnePass = 1, kHalfThree = 2, kHalfOne = 3 };
@@ -136,6 +142,7 @@ struct KParams {
     // 16-bit halves: what split_half_kernel left beside them
     const int *a_exp, *b_exp;              // the operands were multiplied by 2^exponent
     const unsigned int *half_status;       // bit 0: some operand's range did not fit
+    int symmetric;                         // kPolynomial: only tiles on and above the diagonal are computed
 };
 
 // What a launch computes: one product, or (16-bit planes) two that need nothing from each other, the units of the second dealt
@@ -148,6 +155,11 @@ template <int N>
 struct Products {
     Product s[N];
     int count;
+};
+struct FusedProduct {
+    Product s[1];
+    int count;
+    FusedArgs f;
 };
 
 // ------------------------------------------------------------------ PTX helpers
@@ -402,8 +414,22 @@ __device__ __forceinline__ TileCoord decode_unit(const KParams &p, int unit) {
     t.park = 0;
     t.chunk = 0;
     t.tile = tile;
-    const int per_batch = p.tiles_m * p.tiles_n;
     t.bt = fd_div(tile, p.fd_per_batch);
+    if constexpr (TAIL == kPolynomial) {
+        if (p.symmetric) {                         // row tm of the triangle begins at tm * (2T + 1 - tm) / 2
+            const int r = tile - t.bt * static_cast<int>(p.fd_per_batch.d), n = p.tiles_m, b = 2 * n + 1;
+            int tm = static_cast<int>((b - sqrtf(static_cast<float>(b) * b - 8.f * r)) * 0.5f);
+            tm = max(0, min(n - 1, tm));
+            while (tm > 0 && tm * (b - tm) / 2 > r) --tm;
+            while (tm + 1 < n && (tm + 1) * (b - tm - 1) / 2 <= r) ++tm;
+            t.tm = tm;
+            t.tn = tm + (r - tm * (b - tm) / 2);
+            t.it0 = 0;
+            t.it1 = p.fold * p.kiters;
+            return t;
+        }
+    }
+    const int per_batch = p.tiles_m * p.tiles_n;
     const int r = tile - t.bt * per_batch;
     const int group_sz = p.group_m * p.tiles_n;
     const int g = fd_div(r, p.fd_group_sz);
@@ -555,13 +581,16 @@ struct RegShare {
 // ... and of the two-accumulator variant, 168 of 384 threads at launch: two epilogue warpgroups and the one of all other roles.
 constexpr int kTwoEpilogue = 224, kTwoIssue = 56, kTwoLaunch = 168;
 static_assert(2 * kTwoEpilogue + kTwoIssue <= 3 * kTwoLaunch, "more registers than the launch has");
-__host__ __device__ constexpr int product_slots(int mode) { return mode == kHalfThree || mode == kHalfOne ? 2 : 1; }
+__host__ __device__ constexpr int product_slots(int mode, int tail) { return (mode == kHalfThree || mode == kHalfOne) && !is_fused(tail) ? 2 : 1; }
+template <int MODE, int TAIL>
+using KernelArgs = std::conditional_t<is_fused(TAIL), FusedProduct, Products<product_slots(MODE, TAIL)>>;
 template <int BN, int BK, int MODE, int NS, int CG, bool TA = false, int TAIL = kWholeTiles, int SG = 1>
 __global__ void __launch_bounds__(gemm_threads(NS, TAIL == kRunningSum), 1)
-gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
+gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
     const KParams &p = g.s[0].p;                           // what every product of the launch shares is read there
     constexpr bool SK = TAIL == kBalanced, CUT = TAIL == kCutTiles;
     constexpr bool HALF = MODE == kHalfThree || MODE == kHalfOne, FAST = MODE != kThreePass;   // FAST: the split warps split nothing
+    static_assert(!is_fused(TAIL) || MODE == kHalfThree, "fused epilogues are built for products of 16-bit halves");
     static_assert(!HALF || (BN == 256 && BK == 64 && CG == 2 && !TA && !SK), "16-bit halves are built for 256-wide pairs");
     constexpr uint32_t ELT = HALF ? 2 : 4;                 // bytes of a staged element
     constexpr int BNL = BN / CG;                           // B rows staged by this CTA
@@ -658,7 +687,7 @@ gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
     if (p.dep_mode == 1 && threadIdx.x == 0) grid_dependency_trigger();
     // HALF: wide if some operand's range did not fit f16, and the planes hold bf16 thirds, unscaled.
     bool wide = false, huge = false;
-    if constexpr (HALF) {
+    if constexpr (HALF && TAIL != kPolynomial) {       // (its planes are f16 always)
         const unsigned int status = __ldcg(p.half_status);
         wide = (status & 1u) != 0;
         huge = (status & 2u) != 0;
@@ -692,7 +721,7 @@ gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
         const Product &w = g.s[HALF ? prod : 0];
         const KParams &q = HALF ? w.p : p;
         float unscale = 1.f;
-        if constexpr (HALF) {
+        if constexpr (HALF && TAIL != kPolynomial) {
             int ea = __ldcg(q.a_exp), eb = __ldcg(q.b_exp);          // at most 60 either way
             if (wide) { ea = half_wide_exponent(ea, huge); eb = half_wide_exponent(eb, huge); }
             unscale = __uint_as_float(static_cast<uint32_t>(127 - ea - eb) << 23);
@@ -811,6 +840,20 @@ gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
                 if (p.prof) t_ld += clock64() - t_ld0;
                 ++acc_it;
                 if (!last_piece) continue;
+            }
+            if constexpr (is_fused(TAIL)) {
+                const FusedTile at{row0 + lane, q.M, t.tn * BN + chunk_lo * 32, q.N, t.bt, t.tn * 2 + (ew >> 2), t.tm != t.tn, lane};
+                if constexpr (TAIL == kRowStats) {
+                    logit_pairs(g.f, at, run, unscale);
+                    continue;
+                } else if constexpr (TAIL == kRowGrads) {
+                    if (wide) logit_grads<true>(g.f, at, run, unscale);
+                    else logit_grads<false>(g.f, at, run, unscale);
+                    continue;
+                } else {
+                    polynomial(g.f, at, run);
+                    if (!g.f.final) continue;
+                }
             }
             if (row0 < q.M) {
 #pragma unroll(RUN ? CHUNKS : 1)
@@ -1111,7 +1154,7 @@ gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
             const uint32_t dstA0 = smem_u32(stage_base);
             uint32_t dstA = dstA0;
 #pragma unroll                             // parameters at constant addresses, so that what an MMA or a copy takes stays uniform
-            for (int prod = 0; prod < product_slots(MODE); ++prod) {
+            for (int prod = 0; prod < product_slots(MODE, TAIL); ++prod) {
             if (!ok || prod >= products) break;
             const Product &w = g.s[HALF ? prod : 0];
             const KParams &q = HALF ? w.p : p;
@@ -1206,7 +1249,7 @@ gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
             bool next_ready = false;                   // the stage about to be consumed was already seen complete
             const uint32_t sa0 = smem_u32(stage_base);
 #pragma unroll                             // parameters at constant addresses, so that what an MMA or a copy takes stays uniform
-            for (int prod = 0; prod < product_slots(MODE); ++prod) {
+            for (int prod = 0; prod < product_slots(MODE, TAIL); ++prod) {
             if (!ok || prod >= products) break;
             const KParams &q = HALF ? g.s[prod].p : p;
             const uint32_t a_lo0 = ((sa0 >> 4) & 0x3FFFu) | q.a_desc_lbo;
@@ -1382,7 +1425,7 @@ gemm_tc_kernel(const __grid_constant__ Products<product_slots(MODE)> g) {
             constexpr int U = !EXACT ? 1 : (PER % 4 == 0) ? 4 : (PER % 2 == 0 ? 2 : 1);
             if (HALF && warp != SPLIT0) ok = false;           // one warp relays there
 #pragma unroll                             // parameters at constant addresses, so that what an MMA or a copy takes stays uniform
-            for (int prod = 0; prod < product_slots(MODE); ++prod) {
+            for (int prod = 0; prod < product_slots(MODE, TAIL); ++prod) {
             if (!ok || prod >= products) break;
             const KParams &q = HALF ? g.s[prod].p : p;
             WorkIter wi = work_begin(q, first_unit(prod), unit_step);
@@ -1893,7 +1936,7 @@ Cut cut_tail(long long tiles, long long slots, long long k, bool round_only) {
 // activation needs the whole sum in one accumulator.
 constexpr int kHalfChunkK = 4096;
 int chunk_iters_for(const GemmProblem &p, int bk) {
-    const int chunk_k = env_int("MNI_B200_CHUNK_K", p.ha ? kHalfChunkK : 1024);
+    const int chunk_k = env_int("MNI_B200_CHUNK_K", p.chunk_k ? p.chunk_k : p.ha ? kHalfChunkK : 1024);
     return (chunk_k > 0 && p.D == nullptr) ? std::max(1, chunk_k / bk) : 0;
 }
 
@@ -2213,7 +2256,7 @@ uint32_t desc_hi_bits(uint32_t sbo_bytes, uint32_t layout_type) {
 }
 
 template <int BN, int BK, int MODE, int NS, int CG, bool TA = false, int TAIL = kWholeTiles, int SG = 1>
-cudaError_t launch_variant(const Plan &pl, const Product *const *w, int count, cudaStream_t stream) {
+cudaError_t launch_variant(const Plan &pl, const Product *const *w, int count, cudaStream_t stream, const FusedArgs *fused = nullptr) {
     // The shared-memory opt-in is an attribute of the function on ONE device: set once per device of the process
     // (a bit per device ordinal; setting it twice from two threads is harmless).
     static std::atomic<uint64_t> opted_in{0};
@@ -2241,9 +2284,10 @@ cudaError_t launch_variant(const Plan &pl, const Product *const *w, int count, c
     attrs[1].val.clusterDim.z = 1;
     cfg.attrs = attrs;
     cfg.numAttrs = CG == 2 ? 2 : 1;
-    Products<product_slots(MODE)> g;
-    for (int i = 0; i < product_slots(MODE); ++i) g.s[i] = *w[i < count ? i : 0];
+    KernelArgs<MODE, TAIL> g;
+    for (int i = 0; i < product_slots(MODE, TAIL); ++i) g.s[i] = *w[i < count ? i : 0];
     g.count = count;
+    if constexpr (is_fused(TAIL)) g.f = *fused;
     return cudaLaunchKernelEx(&cfg, gemm_tc_kernel<BN, BK, MODE, NS, CG, TA, TAIL, SG>, g);
 }
 
@@ -2659,6 +2703,46 @@ int launch_gemm_halves(const GemmProblem *p, int count, float *const *partial, u
         const int rc = finish[i] ? finish[i](both ? i + 1 : 0, stream) : static_cast<int>(MNI_B200_OK);
         if (rc) return rc;
     }
+    return MNI_B200_OK;
+}
+
+// A product from 16-bit planes with one of the fused epilogues: whole tiles, dealt out round-robin.
+int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, bool symmetric, uint32_t *err_word, int sm_count, cudaStream_t stream) {
+    if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return MNI_B200_OK;
+    const int64_t tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256;
+    const int64_t per_batch = symmetric ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
+    if (p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.K > 0x7fffffffLL || p.batch * per_batch > 0x3fffffffLL || p.batch * tiles_m * tiles_n > 0x3fffffffLL)
+        return fail(MNI_B200_ERR_TOO_LARGE, "product %lld x %lld x %lld (batch %lld) exceeds the kernels' int32 indexing", (long long)p.M,
+                    (long long)p.N, (long long)p.K, (long long)p.batch);
+    Plan pl{};
+    pl.bn = 256;
+    pl.bk = 64;
+    pl.cg = 2;
+    pl.patches = 1;
+    pl.splits = 1;
+    const size_t stage = static_cast<size_t>(BM + 128) * pl.bk * 2, fixed = 1024 + kBarBytes + static_cast<size_t>(kEpiWarps) * kEpiBufBytes;
+    pl.stages = static_cast<int>(std::min<size_t>(kMaxStages, (227 * 1024 - fixed) / stage));
+    pl.smem = fixed + static_cast<size_t>(pl.stages) * stage;
+    pl.tiles_m = static_cast<int>(tiles_m);
+    pl.tiles_n = static_cast<int>(tiles_n);
+    pl.grid = static_cast<int>(std::min<int64_t>(p.batch * per_batch, std::max(1, sm_count / 2))) * 2;
+    Product w;
+    const int rc = make_product(p, pl, false, p.M, p.N, nullptr, err_word, w);
+    if (rc) return rc;
+    if (symmetric) {
+        w.p.symmetric = 1;
+        w.p.fd_per_batch = make_fastdiv(per_batch);
+        w.p.units = static_cast<int>(p.batch * per_batch);
+    }
+    const Product *const products[1] = {&w};
+    cudaError_t e;
+    switch (kind) {
+        case kFusedPairs: e = launch_variant<256, 64, kHalfThree, 2, 2, false, kRowStats>(pl, products, 1, stream, &f); break;
+        case kFusedGrads: e = launch_variant<256, 64, kHalfThree, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f); break;
+        default: e = launch_variant<256, 64, kHalfThree, 2, 2, false, kPolynomial>(pl, products, 1, stream, &f); break;
+    }
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "gemm_tc_kernel set-up failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("gemm_tc_kernel");
     return MNI_B200_OK;
 }
 

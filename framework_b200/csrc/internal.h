@@ -168,6 +168,7 @@ struct GemmProblem {
     // The operands in 16-bit planes (A and B are not read then) and the status word of the launch that made them.
     const HalfOperand *ha = nullptr, *hb = nullptr;
     const unsigned int *half_status = nullptr;
+    int chunk_k = 0;               // longest contraction summed in one accumulator (0: the kernels' own choice)
 };
 
 // Bytes of split-K partial storage launch_gemm_tc would use for this problem (0 if none).
@@ -191,6 +192,33 @@ int launch_gemm_halves(const GemmProblem *p, int count, float *const *partial, u
 void gemm_halves_partial_bytes(const GemmProblem *p, int count, int sm_count, size_t *bytes);
 double gemm_halves_estimate_us(const GemmProblem *p, int count, int sm_count);     // without the pass that makes the planes
 void gemm_halves_describe(const GemmProblem *p, int count, int sm_count, std::string *lines);
+
+// Products from 16-bit planes whose results leave the kernel in another form (fused_epilogue.h).
+enum FusedKind { kFusedPairs, kFusedGrads, kFusedPolynomial };
+struct Targets {
+    const void *ptr;               // whole numbers of `bytes` bytes (4 or 8), one per row; below zero: the row is left out
+    int bytes;
+};
+struct FusedArgs {
+    // logits: this launch's columns are classes first_class .. first_class + N of `classes`
+    Targets targets;
+    int first_class, classes;
+    const float *bias;
+    float2 *pairs;                 // [128 columns][row]
+    float *at_target;              // [row]
+    const float *lse;
+    // planes written: [batch][row][pitch], `matrix` and `plane` elements apart
+    uint16_t *dst;
+    long long dst_pitch, dst_matrix, dst_plane;
+    // polynomial: alpha * product + beta * add, `add` in f16 planes of the result's shape (may be null); final: to the problem's C as f32
+    const uint16_t *add;
+    long long add_pitch, add_matrix, add_plane;
+    float alpha, beta;
+    int final;
+    int mirror;                    // of a symmetric result: tiles above the diagonal are written below it too
+};
+int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, bool symmetric, uint32_t *err_word, int sm_count, cudaStream_t stream);
+constexpr int kGradExponent = 14;      // logit gradients, -1 to 1, are multiplied by 2^14 in f16 planes
 // One line of text naming the kernel variant, tiling, split and grid launch_gemm_tc would use for this problem
 // on a device with `sm_count` SMs.  Pure host arithmetic: touches no device.
 std::string gemm_tc_describe(const GemmProblem &p, int sm_count);
@@ -312,10 +340,6 @@ size_t half_columns_bytes(const HalfView &first, int blocks);
 int launch_split_half(const HalfView *views, int count, int planes, unsigned int *status, int blocks, const HalfColumns &sums,
                       cudaStream_t stream);
 // Softmax cross entropy of a projection (loss.cu).
-struct Targets {
-    const void *ptr;               // whole numbers of `bytes` bytes (4 or 8), one per row; below zero: the row is left out
-    int bytes;
-};
 // The rows of a tensor of up to 8 dims, its last dim the columns.
 struct RowsIn {
     const float *ptr;
@@ -343,7 +367,14 @@ int launch_loss_finish(const float2 *pairs, int64_t parts, int64_t rows, int64_t
 // weights[row] = the row's share in the reduced loss times its gradient; copy (may be null): x, rows left out as zeros, the others
 // multiplied by their weights if `scaled`
 int launch_row_weights(const RowsIn &x, const Targets &targets, int reduction, const float *grad, int *count, float *weights, float *copy,
-                       bool scaled, int sm_count, cudaStream_t stream);
+                       bool scaled, int *grad_exponent, int sm_count, cudaStream_t stream);
+// dx (+)= weights * sums, row by row
+int launch_scale_rows(const float *sums, int64_t ld, const float *weights, float *dx, int64_t rows, int64_t cols, bool accumulate, int sm_count,
+                      cudaStream_t stream);
+// out (+)= column sums of logit gradients in planes, rows multiplied by their weights; status: of the planes of the operands
+size_t grad_column_sums_bytes(int64_t rows, int64_t n, int sm_count);
+int launch_grad_column_sums(const uint16_t *planes, int64_t pitch, int64_t plane, int64_t rows, int64_t n, const float *weights, const unsigned *status,
+                            float *partial, float *out, bool accumulate, int sm_count, cudaStream_t stream);
 // z -> weights * (exp(z - lse) - [class = target])
 int launch_logit_grad(float *z, int64_t rows, int64_t n, const Targets &targets, const float *lse, const float *weights, cudaStream_t stream);
 
@@ -351,18 +382,23 @@ int launch_logit_grad(float *z, int64_t rows, int64_t n, const Targets &targets,
 struct MuonEntry {
     float *param, *momentum;       // null for a matrix that is only made orthogonal
     const float *grad;
-    float *x;                      // the normalised update
-    int64_t n;
+    float *x;                      // the normalised update, then the orthogonal matrix
+    int64_t rows, cols, n;
     float scale;                   // of the update (learning rate included)
 };
 // momentum = mu * momentum + grad, and the sums of squares of the update u = grad + mu * momentum (nesterov) or momentum, or
 // grad where there is no momentum; then x = u / (norm + eps)
 size_t muon_partial_bytes(const MuonEntry *e, int64_t count);
-int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, cudaStream_t stream);
+// Where x goes: f16 planes times 2^exponent, matrix after matrix, or (dst null) to each entry's x in f32.
+struct MuonPlanes {
+    uint16_t *dst = nullptr;
+    int64_t pitch = 0, matrix = 0, plane = 0;
+    int exponent = 0;
+};
+int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, const MuonPlanes &planes,
+                      cudaStream_t stream);
 // param = decay * param - scale * x
 int launch_muon_update(const MuonEntry *e, int64_t count, float decay, cudaStream_t stream);
-// out = alpha * x + beta * y
-int launch_combine(const float *x, const float *y, float *out, int64_t n, float alpha, float beta, cudaStream_t stream);
 // device-side utils::unbroadcast: out[orig] (+)= sum over broadcast dims of grad[gshape]
 int launch_unbroadcast(const float *grad, const int64_t *gshape, int gnd, const int64_t *oshape, int ond,
                        float *out, bool accumulate, cudaStream_t stream);

@@ -12,6 +12,8 @@
 // row's loss, and with it the gradients, NaN: a mistake that shows, where a check would have to wait for the device.
 #include "internal.h"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -194,10 +196,11 @@ count_rows_kernel(Targets targets, int rows, int *count) {
 // whose rows are multiplied by them (scaled), or left out where they are zero.  A block takes rows in turn.
 __global__ void __launch_bounds__(kThreads)
 row_weights_kernel(const __grid_constant__ RowsIn x, Targets targets, int reduction, const float *__restrict__ grad, const int *count,
-                   float *__restrict__ weights, float *__restrict__ copy, int scaled) {
+                   float *__restrict__ weights, float *__restrict__ copy, int scaled, int *grad_exponent) {
     __shared__ int red[32];
     grid_dependency_trigger();
     grid_dependency_wait();
+    if (grad_exponent && blockIdx.x == 0 && threadIdx.x == 0) *grad_exponent = kGradExponent;
     float all = 1.f;
     if (reduction != 0) {
         all = grad[0];
@@ -234,7 +237,112 @@ logit_grad_kernel(float *__restrict__ z, int n, FastDiv stretches, Targets targe
     }
 }
 
+// dx (+)= weights * sums, row by row.
+__global__ void __launch_bounds__(kThreads)
+scale_rows_kernel(const float *__restrict__ sums, int ld, const float *__restrict__ weights, float *__restrict__ dx, long long n, FastDiv cols,
+                  int accumulate) {
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
+        const long long row = n < 0x7fffffffLL ? fd_div(static_cast<int>(i), cols) : i / cols.d;
+        const float w = weights[row];
+        // nothing of a row left out: 0 * NaN would be NaN
+        const float v = w == 0.f ? 0.f : sums[row * ld + (i - row * cols.d)] * w;
+        dx[i] = accumulate ? dx[i] + v : v;
+    }
+}
+
+// Column sums of logit gradients in planes (three bf16 where `status` says so), rows multiplied by their weights: 64 columns and a
+// stretch of rows a block, 8 columns a thread; partial[stretch][columns].
+constexpr int kSumCols = 64;
+__global__ void __launch_bounds__(kThreads)
+grad_column_sums_kernel(const uint16_t *__restrict__ planes, long long pitch, long long plane, int rows, int n, const float *__restrict__ weights,
+                        const unsigned *__restrict__ status, float *__restrict__ partial, int stretch) {
+    __shared__ float red[32][kSumCols];
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const bool wide = (__ldcg(status) & 1u) != 0;
+    const int col = blockIdx.x * kSumCols + (threadIdx.x & 7) * 8, lane_row = threadIdx.x >> 3;
+    const int r0 = blockIdx.y * stretch, r1 = min(rows, r0 + stretch);
+    float sum[8] = {};
+    for (int r = r0 + lane_row; r < r1; r += 32) {
+        const float w = weights[r];
+        const uint16_t *at = planes + r * pitch + col;
+        const uint4 a = __ldcg(reinterpret_cast<const uint4 *>(at)), b = __ldcg(reinterpret_cast<const uint4 *>(at + plane));
+        const unsigned *const x = &a.x, *const y = &b.x;
+        if (wide) {
+            const uint4 d = __ldcg(reinterpret_cast<const uint4 *>(at + 2 * plane));
+            const unsigned *const z = &d.x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                auto part = [i](unsigned v) { return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16); };
+                sum[i] = fmaf(w, part(x[i / 2]) + (part(y[i / 2]) + part(z[i / 2])), sum[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&x[i / 2])), l = __half22float2(*reinterpret_cast<const __half2 *>(&y[i / 2]));
+                constexpr float lo = 1.f / (1 << kHalfLoShift), unit = 1.f / (1 << kGradExponent);
+                sum[i] = fmaf(w, fmaf(l.x, lo, h.x) * unit, sum[i]);
+                sum[i + 1] = fmaf(w, fmaf(l.y, lo, h.y) * unit, sum[i + 1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[lane_row][(threadIdx.x & 7) * 8 + i] = sum[i];
+    __syncthreads();
+    if (threadIdx.x < kSumCols && static_cast<int>(blockIdx.x * kSumCols + threadIdx.x) < n) {
+        float s = red[0][threadIdx.x];
+        for (int r = 1; r < 32; ++r) s += red[r][threadIdx.x];
+        partial[static_cast<long long>(blockIdx.y) * n + blockIdx.x * kSumCols + threadIdx.x] = s;
+    }
+}
+__global__ void __launch_bounds__(kThreads)
+add_stretches_kernel(const float *__restrict__ partial, int stretches, int n, float *__restrict__ out, int accumulate) {
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int c = blockIdx.x * kThreads + threadIdx.x;
+    if (c >= n) return;
+    float s = partial[c];
+    for (int i = 1; i < stretches; ++i) s += partial[static_cast<long long>(i) * n + c];
+    out[c] = accumulate ? out[c] + s : s;
+}
+
 }  // namespace
+
+int launch_scale_rows(const float *sums, int64_t ld, const float *weights, float *dx, int64_t rows, int64_t cols, bool accumulate, int sm_count,
+                      cudaStream_t stream) {
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((rows * cols + kThreads - 1) / kThreads, 8ll * sm_count));
+    const cudaError_t e = launch_dependent(scale_rows_kernel, dim3(blocks), dim3(kThreads), 0, stream, sums, static_cast<int>(ld), weights, dx,
+                                           static_cast<long long>(rows * cols), make_fastdiv(cols), accumulate ? 1 : 0);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "scale_rows_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("scale_rows_kernel");
+    return MNI_B200_OK;
+}
+
+// Rows of a stretch: enough blocks for two rounds of four a SM, 64 stretches at most.
+static int64_t sum_stretch(int64_t rows, int64_t n, int sm_count) {
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(64, 8ll * sm_count / ((n + kSumCols - 1) / kSumCols)));
+    return std::max<int64_t>(32, ((rows + want - 1) / want + 31) / 32 * 32);
+}
+size_t grad_column_sums_bytes(int64_t rows, int64_t n, int sm_count) {
+    const int64_t stretch = sum_stretch(rows, n, sm_count);
+    return static_cast<size_t>((rows + stretch - 1) / stretch * n) * sizeof(float);
+}
+int launch_grad_column_sums(const uint16_t *planes, int64_t pitch, int64_t plane, int64_t rows, int64_t n, const float *weights, const unsigned *status,
+                            float *partial, float *out, bool accumulate, int sm_count, cudaStream_t stream) {
+    const int64_t stretch = sum_stretch(rows, n, sm_count), stretches = (rows + stretch - 1) / stretch;
+    cudaError_t e = launch_dependent(grad_column_sums_kernel, dim3(static_cast<unsigned>((n + kSumCols - 1) / kSumCols), static_cast<unsigned>(stretches)),
+                                     dim3(kThreads), 0, stream, planes, static_cast<long long>(pitch), static_cast<long long>(plane),
+                                     static_cast<int>(rows), static_cast<int>(n), weights, status, partial, static_cast<int>(stretch));
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "grad_column_sums_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("grad_column_sums_kernel");
+    e = launch_dependent(add_stretches_kernel, dim3(static_cast<unsigned>((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, partial,
+                         static_cast<int>(stretches), static_cast<int>(n), out, accumulate ? 1 : 0);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "add_stretches_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("add_stretches_kernel");
+    return MNI_B200_OK;
+}
 
 int launch_logit_stats(const float *z, int64_t rows, int64_t n, const Targets &targets, float2 *pairs, float *at_target, cudaStream_t stream) {
     const int64_t stretches = (n + kStretch - 1) / kStretch;
@@ -263,7 +371,7 @@ int launch_loss_finish(const float2 *pairs, int64_t parts, int64_t rows, int64_t
 }
 
 int launch_row_weights(const RowsIn &x, const Targets &targets, int reduction, const float *grad, int *count, float *weights, float *copy,
-                       bool scaled, int sm_count, cudaStream_t stream) {
+                       bool scaled, int *grad_exponent, int sm_count, cudaStream_t stream) {
     const int *counted = nullptr;
     if (reduction == 2 && x.rows > kCountRows) {
         const cudaError_t e = launch_dependent(count_rows_kernel, dim3(1), dim3(1024), 0, stream, targets, x.rows, count);
@@ -273,7 +381,7 @@ int launch_row_weights(const RowsIn &x, const Targets &targets, int reduction, c
     }
     const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(x.rows, 8ll * sm_count));
     const cudaError_t e = launch_dependent(row_weights_kernel, dim3(blocks), dim3(kThreads), 0, stream, x, targets, reduction, grad, counted,
-                                           weights, copy, scaled ? 1 : 0);
+                                           weights, copy, scaled ? 1 : 0, grad_exponent);
     if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "row_weights_kernel launch failed: %s", cudaGetErrorString(e));
     MNI_LAUNCH_CHECK("row_weights_kernel");
     return MNI_B200_OK;

@@ -9,6 +9,8 @@
 // summed in f64, in a fixed order.
 #include "internal.h"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -26,6 +28,7 @@ struct List {
     const float *grad[kMaxList];
     long long n[kMaxList];
     float scale[kMaxList];
+    int rows[kMaxList], cols[kMaxList];
     unsigned first[kMaxList + 1];              // index of a matrix's first chunk
     int chunk[kMaxList];                       // elements of one
     int count;
@@ -124,12 +127,64 @@ muon_update_kernel(const __grid_constant__ List list, float decay) {
     for (long long i = base + threadIdx.x; i < end; i += kThreads) p[i] = fmaf(-scale, x[i], decay * p[i]);
 }
 
+// x in f16 planes, hi + lo * 2^-12, 8 columns a thread; the matrices of a list are of one shape.  Bound by memory: 8 bytes read (4
+// without a momentum), 4 written.
+struct PlanesOut {
+    uint16_t *dst;
+    long long pitch, matrix, plane;
+    float scale;                               // 2^exponent
+    FastDiv vectors;                           // of a row
+    int first;                                 // index of the list's first matrix
+};
 __global__ void __launch_bounds__(kThreads)
-combine_kernel(const float *x, const float *y, float *out, long long n, float alpha, float beta) {
+muon_planes_kernel(const __grid_constant__ List list, float mu, bool nesterov, float eps, const double *__restrict__ partial, PlanesOut out,
+                   int per_block) {
+    __shared__ double red[8];
     grid_dependency_trigger();
     grid_dependency_wait();
-    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads)
-        out[i] = fmaf(alpha, x[i], beta * y[i]);
+    const int t = blockIdx.y, rows = list.rows[t], cols = list.cols[t];
+    const float factor = inverse_norm(list, t, partial, eps, red) * out.scale;
+    const float *const m = list.momentum[t], *const g = list.grad[t];
+    uint16_t *const dst = out.dst + (out.first + t) * out.matrix;
+    const bool vec = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 && cols % 4 == 0;
+    const int vectors = static_cast<int>(out.vectors.d) * rows, v0 = blockIdx.x * per_block, v1 = min(vectors, v0 + per_block);
+    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+        const int row = fd_div(v, out.vectors), col = (v - row * static_cast<int>(out.vectors.d)) * 8;
+        const long long at = static_cast<long long>(row) * cols + col;
+        float x[8], y[8];
+        if (vec && col + 8 <= cols) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(g + at) + h);
+                x[4 * h] = a.x; x[4 * h + 1] = a.y; x[4 * h + 2] = a.z; x[4 * h + 3] = a.w;
+                if (m) {
+                    const float4 b = __ldcg(reinterpret_cast<const float4 *>(m + at) + h);
+                    y[4 * h] = b.x; y[4 * h + 1] = b.y; y[4 * h + 2] = b.z; y[4 * h + 3] = b.w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = col + i < cols ? __ldg(g + at + i) : 0.f;
+                if (m) y[i] = col + i < cols ? __ldcg(m + at + i) : 0.f;
+            }
+        }
+        uint4 hi, lo;
+        unsigned *const h = &hi.x, *const l = &lo.x;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float a = (m ? update_of(x[i], y[i], mu, nesterov) : x[i]) * factor, b = (m ? update_of(x[i + 1], y[i + 1], mu, nesterov) : x[i + 1]) * factor;
+            const __half2 top = __floats2half2_rn(a, b);
+            const float2 back = __half22float2(top);
+            constexpr float up = 1 << kHalfLoShift;
+            const __half2 rest = __floats2half2_rn((a - back.x) * up, (b - back.y) * up);
+            h[i / 2] = *reinterpret_cast<const unsigned *>(&top);
+            l[i / 2] = *reinterpret_cast<const unsigned *>(&rest);
+        }
+        uint16_t *const to = dst + row * out.pitch + col;
+        *reinterpret_cast<uint4 *>(to) = hi;
+        *reinterpret_cast<uint4 *>(to + out.plane) = lo;
+    }
 }
 
 int64_t chunk_of(int64_t n) {
@@ -154,6 +209,8 @@ int for_lists(const MuonEntry *e, int64_t count, Launch launch) {
             list.grad[k] = e[at].grad;
             list.n[k] = e[at].n;
             list.scale[k] = e[at].scale;
+            list.rows[k] = static_cast<int>(e[at].rows);
+            list.cols[k] = static_cast<int>(e[at].cols);
             list.chunk[k] = static_cast<int>(chunk_of(e[at].n));
             list.first[k] = static_cast<unsigned>(chunks);
             chunks += chunks_of(e[at].n);
@@ -177,7 +234,8 @@ size_t muon_partial_bytes(const MuonEntry *e, int64_t count) {
     return static_cast<size_t>(chunks) * sizeof(double);
 }
 
-int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, cudaStream_t stream) {
+int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, const MuonPlanes &planes,
+                      cudaStream_t stream) {
     int rc = for_lists(e, count, [&](const List &list, unsigned chunks, int64_t before) -> int {
         const cudaError_t r = launch_dependent(muon_momentum_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, partial + before);
         if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_momentum_kernel launch failed: %s", cudaGetErrorString(r));
@@ -185,11 +243,24 @@ int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov
         return MNI_B200_OK;
     });
     if (rc) return rc;
+    int first = 0;
     return for_lists(e, count, [&](const List &list, unsigned chunks, int64_t before) -> int {
-        const cudaError_t r = launch_dependent(muon_normalise_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, eps,
-                                               static_cast<const double *>(partial + before));
-        if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_normalise_kernel launch failed: %s", cudaGetErrorString(r));
-        MNI_LAUNCH_CHECK("muon_normalise_kernel");
+        const double *const sums = partial + before;
+        cudaError_t r;
+        if (planes.dst) {
+            const int64_t row = planes.pitch / 8, vectors = row * list.rows[0];
+            // at least four vectors a thread of a large matrix, and blocks for some rounds where matrices are few
+            const int64_t blocks = std::min<int64_t>((vectors + kThreads - 1) / kThreads, std::max<int64_t>(1, 16ll * device_sm_count() / list.count));
+            const PlanesOut out{planes.dst, planes.pitch, planes.matrix, planes.plane, ldexpf(1.f, planes.exponent), make_fastdiv(row), first};
+            const int per = static_cast<int>(((vectors + blocks - 1) / blocks + kThreads - 1) / kThreads * kThreads);
+            r = launch_dependent(muon_planes_kernel, dim3(static_cast<unsigned>((vectors + per - 1) / per), static_cast<unsigned>(list.count)), dim3(kThreads), 0,
+                                 stream, list, mu, nesterov, eps, sums, out, per);
+        } else {
+            r = launch_dependent(muon_normalise_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, eps, sums);
+        }
+        first += list.count;
+        if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_planes_kernel launch failed: %s", cudaGetErrorString(r));
+        MNI_LAUNCH_CHECK("muon_planes_kernel");
         return MNI_B200_OK;
     });
 }
@@ -201,15 +272,6 @@ int launch_muon_update(const MuonEntry *e, int64_t count, float decay, cudaStrea
         MNI_LAUNCH_CHECK("muon_update_kernel");
         return MNI_B200_OK;
     });
-}
-
-int launch_combine(const float *x, const float *y, float *out, int64_t n, float alpha, float beta, cudaStream_t stream) {
-    if (n == 0) return MNI_B200_OK;
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((n + kThreads - 1) / kThreads, 8ll * device_sm_count()));
-    const cudaError_t e = launch_dependent(combine_kernel, dim3(blocks), dim3(kThreads), 0, stream, x, y, out, n, alpha, beta);
-    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "combine_kernel launch failed: %s", cudaGetErrorString(e));
-    MNI_LAUNCH_CHECK("combine_kernel");
-    return MNI_B200_OK;
 }
 
 }  // namespace mni

@@ -105,7 +105,7 @@ def compare(F, x, w, targets, bias, reduction="mean", need=("dx", "dw", "dbias")
 
 
 SIZES = [(1, 1, 1), (1, 1, 2), (1, 16, 1), (2, 3, 5), (1, 64, 32000), (8, 40, 4097), (9, 64, 300), (16, 256, 2048), (17, 33, 65), (32, 64, 96),
-         (127, 96, 511), (129, 70, 1025), (256, 256, 256), (300, 513, 1000), (1000, 333, 777), (257, 1030, 2049), (40, 2048, 1500)]
+         (127, 96, 511), (129, 70, 1025), (256, 256, 256), (300, 513, 1000), (1000, 333, 777), (257, 1030, 2049), (40, 2048, 1500), (520, 64, 9000)]
 
 
 @pytest.mark.parametrize("rows,k,n", SIZES)

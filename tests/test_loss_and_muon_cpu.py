@@ -50,7 +50,7 @@ def test_flags_of_the_forward_and_null_outputs(lib):
 
 @pytest.mark.parametrize("change,status,text", [
     (dict(g=(4,)), 1, "at least 2D"), (dict(steps=-1), 4, "-1 steps"), (dict(steps=101), 4, "101 steps"), (dict(eps=-1.0), 4, "eps"),
-    (dict(eps=float("nan")), 4, "eps"), (dict(a=float("inf")), 4, "finite"), (dict(c=float("nan")), 4, "finite"), (dict(out=None), 4, "out is null"),
+    (dict(eps=float("nan")), 4, "eps"), (dict(a=float("inf")), 4, "finite"), (dict(c=float("nan")), 4, "finite"), (dict(a=1e8), 4, "larger than 1e9"), (dict(out=None), 4, "out is null"),
     (dict(g=(1 << 30, 1 << 10)), 9, "too large")])
 def test_refusals_of_orthogonalize(lib, change, status, text):
     args = dict(g=(4, 6), out=OK, steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7)
@@ -78,7 +78,7 @@ def test_refusals_of_muon_step(lib):
         assert muon(lib, *arrays, [4], [4]) == 4 and "share memory" in lib.mni_b200_last_error().decode()
     assert lib.mni_b200_muon_step(1, None, None, None, None, None, None, 0.1, 0.9, 1, 0.0, 5, 1.0, 1.0, 1.0, 0.0, None) == 4
     assert muon(lib, [256], [4096], [8192], [0], [4]) == 0          # nothing to do, and nothing touched
-    assert lib.mni_b200_muon_step(0, None, None, None, None, None, None, 0.1, 0.9, 1, 0.0, 5, 1.0, 1.0, 1.0, 0.0, None) == 0
+    assert lib.mni_b200_muon_step(0, None, None, None, None, None, None, 0.1, 0.9, 1, 0.0, 5, 1.5, -0.5, 0.0, 0.0, None) == 0
 
 
 def test_names_of_reductions_and_scales():

@@ -87,7 +87,7 @@ def test_steps(F, steps, shape):
     assert (far <= off).all() and (far <= 4e-6 * (steps + 1) * torch.linalg.matrix_norm(want)).all()
 
 
-@pytest.mark.parametrize("coefficients", [(1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (15.0, -10.0, 1.5), (0.0, 0.0, 0.0), (1.0, 0.0, 0.0), (0.25, 0.0, 1.0)])
+@pytest.mark.parametrize("coefficients", [(1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (3.0, -3.2, 1.2), (0.0, 0.0, 0.0), (1.0, 0.0, 0.0), (0.25, 0.0, 1.0)])
 def test_other_coefficients(F, coefficients):
     """Some that converge to one, some that make the matrix large or small: the scales of the steps follow."""
     g = gradient(4, 150, 90)
