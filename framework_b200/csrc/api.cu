@@ -1350,8 +1350,8 @@ int for_planes(Call &c, const mni_b200_view *&v, mni_b200_view &packed) {
     return MNI_B200_OK;
 }
 
-// Longest contraction in one accumulator of the tensor core, whose adds truncate (7.5e-10 of the sum an element).
-constexpr int kLossChunkK = 1024;
+// Longest contraction of the large terms in one accumulator of the tensor core, whose adds truncate (7.5e-10 of the sum an element).
+constexpr int kLossChunkK = 512, kMuonChunkK = 128;
 
 // z = x . w of the classes first .. first + count, from planes x (view `xi` of h) and w (view `wi`).
 GemmProblem logits_problem(const LossCall &l, const Halves &h, int wi, int64_t first, int64_t count, HalfOperand &x, HalfOperand &w) {
@@ -1559,7 +1559,7 @@ int loss_bwd_planes(Call &c, const LossCall &l, const float *lse, const float *g
             p[n].accumulate = (flags & MNI_B200_ACCUMULATE_DB) != 0;
             ++n;
         }
-        for (int i = 0; i < n; ++i) p[i].chunk_k = kLossChunkK;
+        for (int i = 0; i < n; ++i) p[i].chunk_k = env_int("MNI_B200_DRAIN_K", kLossChunkK);
         if (n) rc = run_halves(c, p, n, h, a, b, nullptr);
         if (rc == MNI_B200_OK && dbias) {
             const size_t part = c.arena.reserve(grad_column_sums_bytes(l.M, count, c.st->sm_count));
@@ -1658,7 +1658,7 @@ int newton_schulz(Call &c, const NewtonSchulz &ns, const std::vector<StepScales>
         p.M = l.rows; p.N = r.rows; p.K = l.kdim;
         p.batch = g.count;
         p.ha = &l; p.hb = &r;
-        p.chunk_k = kLossChunkK;
+        p.chunk_k = kMuonChunkK;
         FusedArgs f{};
         f.alpha = static_cast<float>(alpha);
         f.beta = static_cast<float>(beta);

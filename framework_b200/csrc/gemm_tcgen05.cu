@@ -40,7 +40,11 @@
 //               16 elements), 1.8 -> 0.96 ms.
 // Operands whose range f16 does not hold come as three (two) bf16 planes through the same stages.
 //
-// Three epilogues of kHalfThree keep a product out of memory altogether (fused_epilogue.h): the pairs (maximum, sum of exponentials) of
+//   kHalfDrain  for products that ask for shorter chains (GemmProblem::chunk_k): the large terms leave their accumulator for the
+//               epilogue's registers every chunk_k elements.  Their chain is that long and no longer (the small terms', whose truncation is
+//               2^-12 of it, is the unit), and the pipe, which has small terms to make meanwhile, does not wait.
+//
+// Three epilogues of kHalfDrain keep a product out of memory altogether (fused_epilogue.h): the pairs (maximum, sum of exponentials) of
 // logits, the gradient of logits as planes for the products that follow, and a polynomial in a matrix, planes again.
 //
 // CG = 2: two CTAs of a cluster share a 256 x BN tile (cta_group::2 MMAs issued by the leader).
@@ -85,11 +89,12 @@ constexpr long long kWaitCycles = 4000000000LL;            // default limit of e
 
 enum OperandMode { kKMajor = 0, kMnMultiBox = 1, kMnSingleBox = 2 };
 enum TailMode { kWholeTiles = 0, kBalanced = 1, kCutTiles = 2, kRunningSum = 3, kRowStats = 4, kRowGrads = 5, kPolynomial = 6 };
-// The last three: whole tiles of kHalfThree with an epilogue of their own.
+// The last three: whole tiles of kHalfDrain with an epilogue of their own.
 __host__ __device__ constexpr bool is_fused(int tail) { return tail >= kRowStats; }
 // How a product is computed: operands as f32 (three TF32 passes, or one), or as the 16-bit halves that split_half_kernel has made
 // of them (three passes, or one).
-enum PassMode { kThreePass = 0, kOnePass = 1, kHalfThree = 2, kHalfOne = 3 };
+// kHalfDrain: as kHalfThree, the large terms taken out of their accumulator every few k-blocks.
+enum PassMode { kThreePass = 0, kOnePass = 1, kHalfThree = 2, kHalfOne = 3, kHalfDrain = 4 };
 enum EpilogueMode { kEpiPlainStores = 0, kEpiTmaStore = 1, kEpiTmaReduce = 2, kEpiVectorStores = 3 };
 
 struct KParams {
@@ -581,7 +586,7 @@ struct RegShare {
 // ... and of the two-accumulator variant, 168 of 384 threads at launch: two epilogue warpgroups and the one of all other roles.
 constexpr int kTwoEpilogue = 224, kTwoIssue = 56, kTwoLaunch = 168;
 static_assert(2 * kTwoEpilogue + kTwoIssue <= 3 * kTwoLaunch, "more registers than the launch has");
-__host__ __device__ constexpr int product_slots(int mode, int tail) { return (mode == kHalfThree || mode == kHalfOne) && !is_fused(tail) ? 2 : 1; }
+__host__ __device__ constexpr int product_slots(int mode, int tail) { return (mode == kHalfThree || mode == kHalfOne || mode == kHalfDrain) && !is_fused(tail) ? 2 : 1; }
 template <int MODE, int TAIL>
 using KernelArgs = std::conditional_t<is_fused(TAIL), FusedProduct, Products<product_slots(MODE, TAIL)>>;
 template <int BN, int BK, int MODE, int NS, int CG, bool TA = false, int TAIL = kWholeTiles, int SG = 1>
@@ -589,8 +594,8 @@ __global__ void __launch_bounds__(gemm_threads(NS, TAIL == kRunningSum), 1)
 gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
     const KParams &p = g.s[0].p;                           // what every product of the launch shares is read there
     constexpr bool SK = TAIL == kBalanced, CUT = TAIL == kCutTiles;
-    constexpr bool HALF = MODE == kHalfThree || MODE == kHalfOne, FAST = MODE != kThreePass;   // FAST: the split warps split nothing
-    static_assert(!is_fused(TAIL) || MODE == kHalfThree, "fused epilogues are built for products of 16-bit halves");
+    constexpr bool HALF = MODE == kHalfThree || MODE == kHalfOne || MODE == kHalfDrain, FAST = MODE != kThreePass;   // FAST: the split warps split nothing
+    static_assert(!is_fused(TAIL) || MODE == kHalfDrain, "fused epilogues are built for products of 16-bit halves");
     static_assert(!HALF || (BN == 256 && BK == 64 && CG == 2 && !TA && !SK), "16-bit halves are built for 256-wide pairs");
     constexpr uint32_t ELT = HALF ? 2 : 4;                 // bytes of a staged element
     constexpr int BNL = BN / CG;                           // B rows staged by this CTA
@@ -601,7 +606,10 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
     // whole warpgroups -- TMA and MMA (and two idle), split, epilogue -- that trade registers.
     // TWO: the large and the small terms of a piece in an accumulator each, all of tensor memory; the epilogue takes both into its
     // registers, whole, before anything is stored, and the next piece begins.
-    constexpr bool TWO = MODE == kHalfThree, RUN = TAIL == kRunningSum || TWO;
+    constexpr bool TWO = MODE == kHalfThree || MODE == kHalfDrain, RUN = TAIL == kRunningSum || TWO;
+    // DRAIN: the large terms are taken out of their accumulator every few k-blocks, while the pipe makes small terms, whose own
+    // chain is as long as the unit (its truncation is 2^-12 of the other's).
+    constexpr bool DRAIN = MODE == kHalfDrain;
     static_assert(!RUN || (BN == 256 && CG == 2), "running sums are built for 256-wide pairs");
     constexpr int SPLIT0 = RUN && !TWO ? 4 : 2, EPI0 = SPLIT0 + NS;   // first split and first epilogue warp
     static_assert(!TA || (!FAST && CG == 1 && BK == 32 && NS == 8 && BN <= 128), "unsupported A-from-TMEM variant");
@@ -711,7 +719,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
         constexpr int CHUNKS = BN / 32 / (kEpiWarps / 4);   // ... and take half of the tile's 32-column chunks each
         const int chunk_lo = (ew >> 2) * CHUNKS;
         uint8_t *my_stage = epi_base + ew * p.epi_patches * kEpiBufBytes;
-        int acc_it = 0;
+        int acc_it = 0, unit_it = 0;
         int patch = 0;                                // staging buffer to use next
         int in_flight = 0;                            // bulk groups committed by lane 0 and not yet waited for
         bool ok = true;
@@ -734,10 +742,12 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
         while (ok && work_next<TAIL>(q, wi, t)) {
             const int buf = TWO ? 0 : acc_it & 1;
             const uint32_t acc_phase = TWO ? acc_it & 1 : (acc_it >> 1) & 1;
-            ok = mbar_wait(bar_acc_full + 8u * buf, acc_phase, abort_flag, p.err, 0x500u | buf, waited, timed, p.wait_cycles);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
+            if (!DRAIN) {
+                ok = mbar_wait(bar_acc_full + 8u * buf, acc_phase, abort_flag, p.err, 0x500u | buf, waited, timed, p.wait_cycles);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+            }
             const bool part = CUT && t.part >= 0;            // of the split tail: a raw partial tile, always through TMA
             const bool fuse = q.splits == 1 && !part;
             const bool tma_here = use_tma || part;
@@ -794,7 +804,54 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                     if (j < unit0) ++n_before;
                 }
             }
-            if constexpr (RUN) {
+            if constexpr (DRAIN) {
+                auto wait_full = [&](int slot, uint32_t phase) {
+                    ok = mbar_wait(bar_acc_full + 8u * slot, phase, abort_flag, p.err, 0x500u | slot, waited, timed, p.wait_cycles);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                    __syncwarp();
+                    return ok;
+                };
+                auto release = [&](int slot) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (cta_rank != 0) mbar_arrive_cta(bar_acc_empty + 8u * slot, 0u);
+                        else mbar_arrive(bar_acc_empty + 8u * slot);
+                    }
+                };
+                const uint32_t large = tbase + chunk_lo * 32, small = large + BN;
+                auto take = [&](uint32_t from, float scale, bool add) {
+#pragma unroll
+                    for (int c = 0; c < 2 * CHUNKS; ++c) {
+                        uint32_t x[16];
+                        tmem_ld16_issue(from + c * 16, x);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            uint32_t &r = run[c / 2][(c & 1) * 16 + e];
+                            r = __float_as_uint(fmaf(__uint_as_float(x[e]), scale, add ? __uint_as_float(r) : 0.f));
+                        }
+                    }
+                };
+                if (last_piece) {
+                    if (!wait_full(1, unit_it & 1)) break;
+                    take(small, wide ? 1.f : 1.f / (1 << kHalfLoShift), later_piece);
+                    release(1);
+                    ++unit_it;
+                }
+                if (!wait_full(0, acc_it & 1)) break;
+                if (!last_piece && !later_piece) {
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) tmem_ld32_issue(large + c * 32, run[c]);
+                    tmem_ld_wait();
+                } else {
+                    take(large, 1.f, true);
+                }
+                release(0);
+                ++acc_it;
+                if (!last_piece) continue;
+            } else if constexpr (RUN) {
                 __syncwarp();                          // tcgen05.ld is warp-collective
                 const long long t_ld0 = p.prof ? clock64() : 0;
                 if (!later_piece) {
@@ -1244,6 +1301,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
             int stage = 0;
             uint32_t phase = 0;
             int acc_it = 0;
+            [[maybe_unused]] int unit_it = 0;
             bool ok = true;
             long long waited = 0, waited_acc = 0;
             bool next_ready = false;                   // the stage about to be consumed was already seen complete
@@ -1267,12 +1325,92 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                 const int iters = wt.it1 - wt.it0;
                 const int buf = TWO ? 0 : acc_it & 1;
                 const uint32_t acc_phase = TWO ? acc_it & 1 : (acc_it >> 1) & 1;
-                ok = mbar_wait_warp(bar_acc_empty + 8u * buf, acc_phase ^ 1u, abort_flag, p.err, 0x200u | buf, waited_acc, timed, p.wait_cycles);
-                if (!ok) break;
-                tc_fence_after();
+                if (!DRAIN) {
+                    ok = mbar_wait_warp(bar_acc_empty + 8u * buf, acc_phase ^ 1u, abort_flag, p.err, 0x200u | buf, waited_acc, timed, p.wait_cycles);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * BN);
                 uint32_t accumulate = 0;
-                if constexpr (HALF) {
+                if constexpr (DRAIN) {
+                    // A k-block's small terms come before its large ones, but in a piece's last k-block: its large terms end the piece, and
+                    // while they are taken out of the accumulator the pipe has the small terms of two k-blocks to make.  In a
+                    // unit's last k-block the small terms end first, and are taken out beside the large ones.
+                    const bool first_piece_of_unit = wt.chunk == 0, last_piece_of_unit = wi.piece_it >= wi.piece_end;
+                    uint32_t small_acc = first_piece_of_unit ? 0u : 1u;
+                    auto next = [&] {
+                        if (++stage == p.stages) { stage = 0; phase ^= 1u; a_lo = a_lo0; b_lo = b_lo0; }
+                        else { a_lo += STAGE16; b_lo += STAGE16; }
+                    };
+                    auto k_loop = [&](auto plane_count) {
+                    constexpr int PLANES = decltype(plane_count)::value;
+                    for (int it = 0; it < iters; ++it) {
+                        const bool ends = it + 1 == iters, large_first = ends && !last_piece_of_unit;
+                        ok = mbar_wait_warp(ready0 + 8u * stage, phase, abort_flag, p.err, 0x300u | stage, waited, timed, p.wait_cycles);
+                        if (!ok) break;
+                        const uint32_t hi_stage = static_cast<uint32_t>(stage), ah = a_lo, bh = b_lo;
+                        auto large = [&] {
+                            if (it == 0) {
+                                ok = mbar_wait_warp(bar_acc_empty, acc_phase ^ 1u, abort_flag, p.err, 0x200u, waited_acc, timed, p.wait_cycles);
+                                if (!ok) return;
+                            }
+                            tc_fence_after();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int ks = 0; ks < KSTEPS; ++ks)
+                                    umma_f16_pair(d_tmem, ah + ks * a_ks, a_hi, bh + ks * b_ks, b_hi, idesc, ks == 0 ? accumulate : 1u);
+                                if (ends) umma_commit_pair(bar_acc_full);
+                            }
+                            __syncwarp();
+                        };
+                        if (large_first) {
+                            large();
+                            if (!ok) break;
+                        }
+                        next();
+                        if (it == 0 && first_piece_of_unit) {
+                            ok = mbar_wait_warp(bar_acc_empty + 8u, (unit_it & 1) ^ 1u, abort_flag, p.err, 0x201u, waited_acc, timed, p.wait_cycles);
+                            if (!ok) break;
+                        }
+#pragma unroll
+                        for (int plane = 1; plane < PLANES; ++plane) {
+                            ok = mbar_wait_warp(ready0 + 8u * stage, phase, abort_flag, p.err, 0x300u | stage, waited, timed, p.wait_cycles);
+                            if (!ok) break;
+                            tc_fence_after();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int ks = 0; ks < KSTEPS; ++ks) {
+                                    umma_f16_pair(d_tmem + BN, a_lo + ks * a_ks, a_hi, bh + ks * b_ks, b_hi, idesc, ks == 0 ? small_acc : 1u);
+                                    umma_f16_pair(d_tmem + BN, ah + ks * a_ks, a_hi, b_lo + ks * b_ks, b_hi, idesc, 1u);
+                                    if (PLANES == 3 && plane == 1)
+                                        umma_f16_pair(d_tmem + BN, a_lo + ks * a_ks, a_hi, b_lo + ks * b_ks, b_hi, idesc, 1u);
+                                }
+                                umma_commit_pair(bar_empty + 8u * stage);
+                                if (plane + 1 == PLANES) {
+                                    if (large_first) umma_commit_pair(bar_empty + 8u * hi_stage);
+                                    if (ends && last_piece_of_unit) umma_commit_pair(bar_acc_full + 8u);
+                                }
+                            }
+                            __syncwarp();
+                            small_acc = 1u;
+                            next();
+                        }
+                        if (!ok) break;
+                        if (!large_first) {
+                            large();
+                            if (!ok) break;
+                            if (elect_one()) umma_commit_pair(bar_empty + 8u * hi_stage);
+                            __syncwarp();
+                        }
+                        accumulate = 1u;
+                    }
+                    };
+                    if (wide) k_loop(std::integral_constant<int, 3>{});
+                    else k_loop(std::integral_constant<int, 2>{});
+                    if (!ok) break;
+                    ++acc_it;
+                    if (last_piece_of_unit) ++unit_it;
+                } else if constexpr (HALF) {
                     auto next = [&] {
                         if (++stage == p.stages) { stage = 0; phase ^= 1u; a_lo = a_lo0; b_lo = b_lo0; }
                         else { a_lo += STAGE16; b_lo += STAGE16; }
@@ -2682,7 +2820,10 @@ int launch_gemm_halves(const GemmProblem *p, int count, float *const *partial, u
     }
     const Plan &pl = pls[0];
     cudaError_t e;
-    if (!p[0].fast_tf32) {
+    if (!p[0].fast_tf32 && p[0].chunk_k > 0) {
+        e = cut ? launch_variant<256, 64, kHalfDrain, 2, 2, false, kCutTiles>(pl, products, count, stream)
+                : launch_variant<256, 64, kHalfDrain, 2, 2>(pl, products, count, stream);
+    } else if (!p[0].fast_tf32) {
         e = cut ? launch_variant<256, 64, kHalfThree, 2, 2, false, kCutTiles>(pl, products, count, stream)
                 : launch_variant<256, 64, kHalfThree, 2, 2>(pl, products, count, stream);
     } else if (cut) {
@@ -2737,9 +2878,9 @@ int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, 
     const Product *const products[1] = {&w};
     cudaError_t e;
     switch (kind) {
-        case kFusedPairs: e = launch_variant<256, 64, kHalfThree, 2, 2, false, kRowStats>(pl, products, 1, stream, &f); break;
-        case kFusedGrads: e = launch_variant<256, 64, kHalfThree, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f); break;
-        default: e = launch_variant<256, 64, kHalfThree, 2, 2, false, kPolynomial>(pl, products, 1, stream, &f); break;
+        case kFusedPairs: e = launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowStats>(pl, products, 1, stream, &f); break;
+        case kFusedGrads: e = launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f); break;
+        default: e = launch_variant<256, 64, kHalfDrain, 2, 2, false, kPolynomial>(pl, products, 1, stream, &f); break;
     }
     if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "gemm_tc_kernel set-up failed: %s", cudaGetErrorString(e));
     MNI_LAUNCH_CHECK("gemm_tc_kernel");

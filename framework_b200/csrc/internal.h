@@ -168,7 +168,7 @@ struct GemmProblem {
     // The operands in 16-bit planes (A and B are not read then) and the status word of the launch that made them.
     const HalfOperand *ha = nullptr, *hb = nullptr;
     const unsigned int *half_status = nullptr;
-    int chunk_k = 0;               // longest contraction summed in one accumulator (0: the kernels' own choice)
+    int chunk_k = 0;               // 16-bit planes: longest contraction of the large terms in one accumulator (0: the kernels' own choice)
 };
 
 // Bytes of split-K partial storage launch_gemm_tc would use for this problem (0 if none).
