@@ -1370,7 +1370,9 @@ GemmProblem logits_problem(const LossCall &l, const Halves &h, int wi, int64_t f
 int loss_fwd_body(Call &c, const LossCall &l, float *loss, float *lse) {
     if (l.M == 0) return MNI_B200_OK;
     const bool planes = loss_from_planes(l);
-    const int64_t stretch = planes ? 128 : kLogitStretch, stretches = (l.N + stretch - 1) / stretch;
+    GemmProblem shape;
+    shape.M = l.M; shape.N = l.N; shape.K = l.K;
+    const int64_t stretch = planes ? fused_stretch(shape, c.gemm_sms()) : kLogitStretch, stretches = (l.N + stretch - 1) / stretch;
     if (!planes && l.M * stretches > 0x7fffffffLL)
         return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld classes are too many", (long long)l.M, (long long)l.N);
     const size_t pairs_at = c.arena.reserve(static_cast<size_t>(stretches * l.M) * sizeof(float2));
@@ -1591,19 +1593,19 @@ struct NewtonSchulz {
 };
 
 // What the matrices of a step can hold at most, so that their planes' exponents need no pass over the data: singular values s of x
-// lie in [0, top] at first 1, A = x x^T holds s^2, Q = b A + c A^2 holds b t + c t^2 of t = s^2, the next x holds s (a + b t + c t^2).
-// No element of a matrix is larger than its largest singular value.
+// lie in [0, top], at first 1; with t = s^2, A = x x^T holds t, R = b + c A holds b + c t, Q = a + A R holds a + b t + c t^2, and the next
+// x is Q x.  No element of a matrix is larger than its largest singular value.
 struct StepScales {
-    int x, a, q;                   // exponents of the planes of x, A, Q
+    int x, a, r, q;                // exponents of the planes of x, A, R, Q
 };
 int step_scales(const NewtonSchulz &ns, std::vector<StepScales> &out) {
     constexpr double kRounding = 1.01;
     auto exponent = [](double bound) { return bound > 0 ? std::max(-40, std::min(40, 15 - static_cast<int>(std::ceil(std::log2(bound))))) : 0; };
     double top = kRounding;
     for (int k = 0; k < ns.steps; ++k) {
-        const double t = top * top;
-        auto q = [&](double y) { return std::fabs(ns.b * y + ns.c * y * y); };
-        double most_q = std::max(q(t), 1e-30);
+        const double t = top * top, most_r = std::max({std::fabs(ns.b), std::fabs(ns.b + ns.c * t), 1e-30});
+        auto q = [&](double y) { return std::fabs(ns.a + ns.b * y + ns.c * y * y); };
+        double most_q = std::max({q(0), q(t), 1e-30});
         if (ns.c != 0 && -ns.b / (2 * ns.c) > 0 && -ns.b / (2 * ns.c) < t) most_q = std::max(most_q, q(-ns.b / (2 * ns.c)));
         auto p = [&](double y) { return std::sqrt(y) * std::fabs(ns.a + ns.b * y + ns.c * y * y); };
         double most_p = p(t);
@@ -1617,9 +1619,9 @@ int step_scales(const NewtonSchulz &ns, std::vector<StepScales> &out) {
                 if (y > 0 && y < t) most_p = std::max(most_p, p(y));
             }
         }
-        out.push_back(StepScales{exponent(top), exponent(t), exponent(most_q)});
+        out.push_back(StepScales{exponent(top), exponent(t), exponent(most_r), exponent(most_q)});
         top = kRounding * std::max(most_p, 1e-30);
-        if (!(top < 1e9) || !(most_q < 1e9))
+        if (!(top < 1e9) || !(most_q < 1e9) || !(most_r < 1e9))
             return fail(MNI_B200_ERR_ARG, "with these coefficients step %d can make singular values larger than 1e9", k + 1);
     }
     return MNI_B200_OK;
@@ -1628,7 +1630,7 @@ int step_scales(const NewtonSchulz &ns, std::vector<StepScales> &out) {
 // Steps on `count` matrices of one shape, from planes (x[0] holds the start) to f32 `out` [count][rows][cols].
 struct MuonGroup {
     int64_t rows, cols, side, count;
-    int64_t x_pitch, x_matrix, s_pitch, s_matrix;          // of x, and of A and Q
+    int64_t x_pitch, x_matrix, s_pitch, s_matrix;          // of x, and of A, R and Q
     MuonGroup(int64_t r, int64_t c, int64_t n)
         : rows(r), cols(c), side(std::min(r, c)), count(n), x_pitch(round_up(c, 64)), x_matrix(r * x_pitch), s_pitch(round_up(side, 64)),
           s_matrix(side * s_pitch) {}
@@ -1636,7 +1638,7 @@ struct MuonGroup {
     size_t s_bytes() const { return static_cast<size_t>(count * s_matrix) * 4; }
 };
 int newton_schulz(Call &c, const NewtonSchulz &ns, const std::vector<StepScales> &scales, const MuonGroup &g, uint16_t *const (&x)[2], uint16_t *a,
-                  uint16_t *q, float *out) {
+                  uint16_t *r, uint16_t *q, float *out) {
     const bool tall = g.rows > g.cols;
     auto operand = [&](const uint16_t *p, bool of_x, bool k_major) {
         HalfOperand o;
@@ -1652,46 +1654,43 @@ int newton_schulz(Call &c, const NewtonSchulz &ns, const std::vector<StepScales>
         o.planes = 2;
         return o;
     };
-    auto product = [&](const HalfOperand &l, const HalfOperand &r, const uint16_t *add, bool add_x, double alpha, double beta, uint16_t *dst, bool dst_x,
-                       float *final_out) {
+    auto product = [&](const HalfOperand &l, const HalfOperand &r, bool square, std::initializer_list<FusedArgs::Output> outputs, float *final_out) {
         GemmProblem p;
         p.M = l.rows; p.N = r.rows; p.K = l.kdim;
         p.batch = g.count;
         p.ha = &l; p.hb = &r;
         p.chunk_k = kMuonChunkK;
         FusedArgs f{};
-        f.alpha = static_cast<float>(alpha);
-        f.beta = static_cast<float>(beta);
-        f.add = add;
-        f.add_pitch = add_x ? g.x_pitch : g.s_pitch;
-        f.add_matrix = add_x ? g.x_matrix : g.s_matrix;
-        f.add_plane = f.add_matrix * g.count;
-        f.dst = dst;
-        f.dst_pitch = dst_x ? g.x_pitch : g.s_pitch;
-        f.dst_matrix = dst_x ? g.x_matrix : g.s_matrix;
+        std::copy(outputs.begin(), outputs.end(), f.out);
+        f.outputs = final_out ? 0 : static_cast<int>(outputs.size());
+        f.dst_pitch = square ? g.s_pitch : g.x_pitch;
+        f.dst_matrix = square ? g.s_matrix : g.x_matrix;
         f.dst_plane = f.dst_matrix * g.count;
+        f.mirror = square ? 1 : 0;
         if (final_out) {
-            f.final = 1;
             p.C = final_out;
             p.ldc = g.cols;
             p.c_bstride = g.rows * g.cols;
         }
-        f.mirror = dst_x ? 0 : 1;
-        return launch_gemm_fused(p, kFusedPolynomial, f, !dst_x, c.st->err_word, c.gemm_sms(), c.stream);
+        return launch_gemm_fused(p, kFusedPolynomial, f, square, c.st->err_word, c.gemm_sms(), c.stream);
     };
+    auto power = [](int e) { return std::ldexp(1.0, e); };
     for (int k = 0; k < ns.steps; ++k) {
         const StepScales &e = scales[static_cast<size_t>(k)];
         const bool last = k + 1 == ns.steps;
         const int next = last ? 0 : scales[static_cast<size_t>(k) + 1].x;
         uint16_t *const from = x[k & 1], *const to = x[(k + 1) & 1];
-        // A = x x^T, or x^T x; the operands are the same planes
-        const HalfOperand xs = operand(from, true, !tall), as = operand(a, false, true), qs = operand(q, false, true);
-        int rc = product(xs, xs, nullptr, false, std::ldexp(1.0, e.a - 2 * e.x), 0.0, a, false, nullptr);
-        if (rc == MNI_B200_OK) rc = product(as, as, a, false, std::ldexp(ns.c, e.q - 2 * e.a), std::ldexp(ns.b, e.q - e.a), q, false, nullptr);
+        // A = x x^T or x^T x (its operands are the same planes), and R = b + c A
+        const HalfOperand xs = operand(from, true, !tall), as = operand(a, false, true), rs = operand(r, false, true), qs = operand(q, false, true);
+        int rc = product(xs, xs, true, {{a, static_cast<float>(power(e.a - 2 * e.x)), 0.f},
+                                        {r, static_cast<float>(ns.c * power(e.r - 2 * e.x)), static_cast<float>(ns.b * power(e.r))}}, nullptr);
+        // Q = a + A R: symmetric, as R is a polynomial in A
+        if (rc == MNI_B200_OK)
+            rc = product(as, rs, true, {{q, static_cast<float>(power(e.q - e.a - e.r)), static_cast<float>(ns.a * power(e.q))}}, nullptr);
         if (rc) return rc;
-        const double alpha = std::ldexp(1.0, next - e.q - e.x), beta = std::ldexp(ns.a, next - e.x);
-        if (tall) rc = product(operand(from, true, true), qs, from, true, alpha, beta, to, true, last ? out : nullptr);      // x Q
-        else rc = product(qs, operand(from, true, false), from, true, alpha, beta, to, true, last ? out : nullptr);          // Q x
+        const FusedArgs::Output out_x{to, static_cast<float>(power(next - e.q - e.x)), 0.f};
+        if (tall) rc = product(operand(from, true, true), qs, false, {out_x}, last ? out : nullptr);      // x Q
+        else rc = product(qs, operand(from, true, false), false, {out_x}, last ? out : nullptr);          // Q x
         if (rc) return rc;
     }
     return MNI_B200_OK;
@@ -1715,7 +1714,7 @@ int muon_body(Call &c, const std::vector<MuonEntry> &e, const NewtonSchulz &ns, 
         const MuonGroup one(all[0].rows, all[0].cols, 1);
         const bool update = all[0].param != nullptr;
         if (one.x_matrix / 8 > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "a matrix of %lld x %lld is too large", (long long)one.rows, (long long)one.cols);
-        const size_t each = 2 * one.x_bytes() + 2 * one.s_bytes() + (update ? static_cast<size_t>(one.rows * one.cols) * 4 : 0);
+        const size_t each = 2 * one.x_bytes() + 3 * one.s_bytes() + (update ? static_cast<size_t>(one.rows * one.cols) * 4 : 0);
         const int64_t at_once = std::max<int64_t>(1, std::min<int64_t>(65535, static_cast<int64_t>(kMuonScratch / each)));
         for (size_t first = 0; first < all.size(); first += static_cast<size_t>(at_once)) {
             const int64_t count = std::min<int64_t>(at_once, static_cast<int64_t>(all.size() - first));
@@ -1723,7 +1722,7 @@ int muon_body(Call &c, const std::vector<MuonEntry> &e, const NewtonSchulz &ns, 
             const MuonGroup g(one.rows, one.cols, count);
             const size_t mark = c.arena.used;
             const size_t sums = c.arena.reserve(muon_partial_bytes(part, count)), x0 = c.arena.reserve(g.x_bytes()), x1 = c.arena.reserve(g.x_bytes()),
-                         a = c.arena.reserve(g.s_bytes()), q = c.arena.reserve(g.s_bytes()),
+                         a = c.arena.reserve(g.s_bytes()), r = c.arena.reserve(g.s_bytes()), q = c.arena.reserve(g.s_bytes()),
                          result = update ? c.arena.reserve(static_cast<size_t>(count * g.rows * g.cols) * 4) : 0;
             c.arena.used = mark;
             if (c.dry()) continue;
@@ -1740,7 +1739,8 @@ int muon_body(Call &c, const std::vector<MuonEntry> &e, const NewtonSchulz &ns, 
             int rc = launch_muon_start(part, count, mu, nesterov, eps, reinterpret_cast<double *>(c.at(sums)), planes, c.stream);
             uint16_t *const x[2] = {reinterpret_cast<uint16_t *>(c.at(x0)), reinterpret_cast<uint16_t *>(c.at(x1))};
             if (rc == MNI_B200_OK)
-                rc = newton_schulz(c, ns, scales, g, x, reinterpret_cast<uint16_t *>(c.at(a)), reinterpret_cast<uint16_t *>(c.at(q)), part[0].x);
+                rc = newton_schulz(c, ns, scales, g, x, reinterpret_cast<uint16_t *>(c.at(a)), reinterpret_cast<uint16_t *>(c.at(r)),
+                                   reinterpret_cast<uint16_t *>(c.at(q)), part[0].x);
             if (rc == MNI_B200_OK && update) rc = launch_muon_update(part, count, decay, c.stream);
             if (rc) return rc;
         }

@@ -1,11 +1,15 @@
-// Epilogues of products from 16-bit planes that never leave their result in memory as f32.  Each epilogue thread holds 128
-// neighbouring columns of one row of a 256 x 256 tile in registers when they begin, and the tensor pipe is at the next tile already.
+// Epilogues of products from 16-bit planes that never leave their result in memory as f32.  A thread holds columns of one row of the
+// tile in registers when they begin, 32 of them a chunk, and the tensor pipe is at the next tile already.
 //
-//   logit_pairs   z = product + bias -> (maximum, sum of exponentials) of the 128 columns, and the target's logit: 8 bytes for 128
-//                 logits instead of 512 written and read again
-//   logit_grads   z -> exp(z - lse) - [class = target], in planes for the two products that follow: 4 bytes instead of 4 + 4 + 4 + 4
+//   PairSum       z = product + bias -> (maximum, sum of exponentials) of a thread's columns, and the target's logit: 8 bytes for
+//                 128 logits instead of 512 written and read again
+//   grad_chunk    z -> exp(z - lse) - [class = target], in planes for the two products that follow: 4 bytes instead of 4 + 4 + 4 + 4
 //                 through f32 logits, f32 gradients and a pass that splits them
-//   polynomial    alpha * product + beta * add -> planes, above and below the diagonal where the result is symmetric
+//   power_chunk   alpha * product + beta * identity -> planes, below the diagonal too where only tiles above it are computed; and
+//                 the same once more with other factors
+//
+// The kernel calls them chunk after chunk in a loop that is not unrolled, and moves the registers down in between: unrolled over 128
+// columns their code (40 KB, executed once a tile) came from beyond the instruction caches, and a tile's epilogue took 12 us.
 //
 // Planes are written row by row, 32 bytes a store of one thread: whole sectors.  Scales are fixed, not looked for: a gradient of
 // logits is at most one, what a polynomial makes is bounded on the host.
@@ -22,76 +26,92 @@ struct FusedTile {
     int row, rows;                 // this thread's row, of so many
     int col, cols;                 // its first column, of so many
     int batch;
-    int stretch;                   // index of the 128 columns
+    int stretch;                   // index of its columns' stretch
     bool off_diagonal;
     int lane;
+    float *patch;                  // 4 KB of shared memory of the warp's own
 };
 
-__device__ __forceinline__ long long fused_target(const Targets &t, int row) {
-    return t.bytes == 8 ? __ldg(static_cast<const long long *>(t.ptr) + row) : __ldg(static_cast<const int *>(t.ptr) + row);
+__device__ __forceinline__ float exp2_approx(float x) {     // 2 ulp; results below 2^-126 are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
+constexpr float kLog2e = 1.4426950408889634f;
 
-// z = x * unscale + bias; columns past the last: -inf.
-__device__ __forceinline__ void logits_of(const FusedArgs &f, const FusedTile &at, uint32_t (&run)[4][32], float unscale) {
-    const bool whole = at.col + 128 <= at.cols;
-    if (!f.bias && whole) {
+// What is added to the logits of a chunk, in the warp's patch: bias, -inf past the last column.  Returns whether there is anything.
+__device__ __forceinline__ bool stage_bias(const FusedArgs &f, const FusedTile &at, int col) {
+    if (!f.bias && col + 32 <= at.cols) return false;
+    const int j = col + at.lane;
+    __syncwarp();
+    at.patch[at.lane] = j < at.cols ? (f.bias ? __ldg(f.bias + f.first_class + j) : 0.f) : -INFINITY;
+    __syncwarp();
+    return true;
+}
+// z = x * unscale (+ the patch)
+__device__ __forceinline__ void logits_of(bool biased, const FusedTile &at, uint32_t (&v)[32], float unscale) {
+    if (biased) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) run[c][e] = __float_as_uint(__uint_as_float(run[c][e]) * unscale);
-        return;
-    }
-    const float *const bias = f.bias + f.first_class + at.col;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            const int j = c * 32 + e;
-            const bool there = at.col + j < at.cols;
-            const float b = f.bias && there ? __ldg(bias + j) : 0.f;
-            run[c][e] = __float_as_uint(there ? fmaf(__uint_as_float(run[c][e]), unscale, b) : -INFINITY);
+        for (int e = 0; e < 32; e += 4) {
+            const float4 b = *reinterpret_cast<const float4 *>(at.patch + e);
+            v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), unscale, b.x));
+            v[e + 1] = __float_as_uint(fmaf(__uint_as_float(v[e + 1]), unscale, b.y));
+            v[e + 2] = __float_as_uint(fmaf(__uint_as_float(v[e + 2]), unscale, b.z));
+            v[e + 3] = __float_as_uint(fmaf(__uint_as_float(v[e + 3]), unscale, b.w));
         }
-}
-
-__device__ __forceinline__ void logit_pairs(const FusedArgs &f, const FusedTile &at, uint32_t (&run)[4][32], float unscale) {
-    if (at.col >= at.cols) return;                 // the same for the whole warp
-    logits_of(f, at, run, unscale);
-    const bool live = at.row < at.rows;
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    } else {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) m[c] = fmaxf(m[c], __uint_as_float(run[c][e]));
-    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    const float shift = isinf(top) ? 0.f : top;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[c] += exp2f((__uint_as_float(run[c][e]) - shift) * 1.44269504f);
-    if (live) f.pairs[static_cast<long long>(at.stretch) * at.rows + at.row] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
-    // the target's logit, in the few tiles that hold one of these rows'
-    const long long t = live ? fused_target(f.targets, at.row) - f.first_class - at.col : -1;
-    const bool mine = t >= 0 && t < 128 && at.col + t < at.cols;
-    if (__any_sync(0xffffffffu, mine)) {
-        float z = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) z = t == c * 32 + e ? __uint_as_float(run[c][e]) : z;
-        if (mine) f.at_target[at.row] = z;
+        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * unscale);
     }
 }
+// The target of a thread's row, relative to column `col` of the launch; anything negative where it is not there.
+__device__ __forceinline__ long long target_of(const FusedArgs &f, const FusedTile &at) {
+    const Targets &t = f.targets;
+    return t.bytes == 8 ? __ldg(static_cast<const long long *>(t.ptr) + at.row) : __ldg(static_cast<const int *>(t.ptr) + at.row);
+}
 
-__device__ __forceinline__ void store_planes16(uint16_t *at, const uint32_t (&v)[8]) {
+struct PairSum {
+    float m, s;
+    int rel;                       // the target, relative to the thread's first column (-1: elsewhere)
+    __device__ __forceinline__ void begin(const FusedArgs &f, const FusedTile &at, int columns) {
+        m = -INFINITY;
+        s = 0.f;
+        const long long t = at.row < at.rows ? target_of(f, at) - f.first_class - at.col : -1;
+        rel = t >= 0 && t < columns && at.col + t < at.cols ? static_cast<int>(t) : -1;
+    }
+    __device__ __forceinline__ void chunk(const FusedArgs &f, const FusedTile &at, uint32_t (&v)[32], int c, float unscale) {
+        const int col = at.col + 32 * c;
+        if (col >= at.cols) return;                // the same for the whole warp
+        logits_of(stage_bias(f, at, col), at, v, unscale);
+        float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(v[e]));
+        const float next = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float shift = isinf(next) ? 0.f : next;
+        float sum[4] = {m == next || m == -INFINITY ? s : s * exp2_approx((m - shift) * kLog2e), 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sum[e & 3] += exp2_approx((__uint_as_float(v[e]) - shift) * kLog2e);
+        m = next;
+        s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // the target's logit, in the few chunks that hold one of these rows'
+        const int r = rel - 32 * c;
+        const bool mine = static_cast<unsigned>(r) < 32u;
+        if (__any_sync(0xffffffffu, mine)) {
+            float z = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) z = r == e ? __uint_as_float(v[e]) : z;
+            if (mine) f.at_target[at.row] = z;
+        }
+    }
+    __device__ __forceinline__ void end(const FusedArgs &f, const FusedTile &at) const {
+        if (at.col < at.cols && at.row < at.rows) f.pairs[static_cast<long long>(at.stretch) * at.rows + at.row] = make_float2(m, s);
+    }
+};
+
+__device__ __forceinline__ void store_planes16(uint16_t *at, const uint32_t *v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                  "r"(v[6]), "r"(v[7])
                  : "memory");
-}
-__device__ __forceinline__ void load_planes16(const uint16_t *at, uint32_t (&v)[8]) {
-    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "l"(at));
 }
 // x = hi + lo * 2^-kHalfLoShift, two elements
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint32_t &lo) {
@@ -103,103 +123,112 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint3
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// WIDE: as three bf16, unscaled, for operands whose range f16 does not hold (an MMA's two operands have one type).
-template <bool WIDE>
-__device__ __forceinline__ void logit_grads(const FusedArgs &f, const FusedTile &at, uint32_t (&run)[4][32], float unscale) {
-    if (at.col >= f.dst_pitch || at.row >= at.rows) return;
-    logits_of(f, at, run, unscale);
-    const float lse = __ldg(f.lse + at.row);
-    const long long t = fused_target(f.targets, at.row);
-    const long long rel = t - f.first_class - at.col;
+struct GradRow {
+    float lse, scale;
+    int rel;
+    bool kept, live;
     // a row left out has no gradient, whatever it holds; a target that is no class makes its row's NaN
-    const float scale = t < f.classes ? (WIDE ? 1.f : static_cast<float>(1 << kGradExponent)) : NAN;
-    uint16_t *const dst = f.dst + at.row * f.dst_pitch + at.col;
+    __device__ __forceinline__ void begin(const FusedArgs &f, const FusedTile &at, bool wide) {
+        live = at.row < at.rows;
+        const long long t = live ? target_of(f, at) : -1, r = t - f.first_class - at.col;
+        lse = live ? __ldg(f.lse + at.row) : 0.f;
+        kept = t >= 0;
+        scale = t < f.classes ? (wide ? 1.f : static_cast<float>(1 << kGradExponent)) : NAN;
+        rel = r >= 0 && r < (1 << 20) ? static_cast<int>(r) : -1;
+    }
+};
+// wide: as three bf16, unscaled, for operands whose range f16 does not hold (an MMA's two operands have one type).
+__device__ __forceinline__ void grad_chunk(const FusedArgs &f, const FusedTile &at, const GradRow &g, uint32_t (&v)[32], int c, float unscale, bool wide) {
+    const int col = at.col + 32 * c;
+    if (col >= f.dst_pitch) return;                // the same for the whole warp; pitches are multiples of 64
+    logits_of(stage_bias(f, at, col), at, v, unscale);
+    const int r = g.rel - 32 * c;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int e = 0; e < 32; ++e) {
+        // the product with log2(e) carried out to where its rounding does not show: an error of 2^-24 of it would be one of the result
+        const float u = __uint_as_float(v[e]) - g.lse, d = u < -200.f ? -200.f : u, y = d * kLog2e;      // (NaN stays)
+        const float p = exp2_approx(y) * fmaf(fmaf(d, kLog2e, -y), 0.6931472f, 1.f);
+        const float x = (e == r ? p - 1.f : p) * g.scale;
+        v[e] = __float_as_uint(g.kept ? x : 0.f);
+    }
+    if (!g.live) return;
+    uint16_t *const dst = f.dst + at.row * f.dst_pitch + col;
+    if (wide) {
+#pragma unroll 1
+        for (int plane = 0; plane < 3; ++plane) {
+            uint32_t x[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int j0 = c * 32 + h * 16;
-            if (at.col + j0 >= f.dst_pitch) return;
-            float d[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = expf(__uint_as_float(run[c][h * 16 + e]) - lse) - (rel == j0 + e ? 1.f : 0.f);
-                d[e] = t >= 0 && at.col + j0 + e < at.cols ? p * scale : 0.f;
+            for (int e = 0; e < 32; e += 2) {
+                const uint32_t a = v[e] & 0xffff0000u, b = v[e + 1] & 0xffff0000u;
+                x[e / 2] = (a >> 16) | b;
+                v[e] = __float_as_uint(__uint_as_float(v[e]) - __uint_as_float(a));
+                v[e + 1] = __float_as_uint(__uint_as_float(v[e + 1]) - __uint_as_float(b));
             }
-            uint32_t x[3][8];
-            if constexpr (WIDE) {
-#pragma unroll
-                for (int plane = 0; plane < 3; ++plane) {
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const uint32_t a = __float_as_uint(d[e]) & 0xffff0000u, b = __float_as_uint(d[e + 1]) & 0xffff0000u;
-                        x[plane][e / 2] = (a >> 16) | b;
-                        d[e] -= __uint_as_float(a);
-                        d[e + 1] -= __uint_as_float(b);
-                    }
-                    store_planes16(dst + plane * f.dst_plane + j0, x[plane]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) split_pair(d[e], d[e + 1], x[0][e / 2], x[1][e / 2]);
-                store_planes16(dst + j0, x[0]);
-                store_planes16(dst + f.dst_plane + j0, x[1]);
-            }
+            store_planes16(dst + plane * f.dst_plane, x);
+            store_planes16(dst + plane * f.dst_plane + 16, x + 8);
         }
+        return;
+    }
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) split_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), hi[e / 2], lo[e / 2]);
+    store_planes16(dst, hi);
+    store_planes16(dst + 16, hi + 8);
+    store_planes16(dst + f.dst_plane, lo);
+    store_planes16(dst + f.dst_plane + 16, lo + 8);
 }
 
-__device__ __forceinline__ void polynomial(const FusedArgs &f, const FusedTile &at, uint32_t (&run)[4][32]) {
-    const bool live = at.row < at.rows;
-    const uint16_t *const add = f.add + at.batch * f.add_matrix + at.row * f.add_pitch + at.col;
-    uint16_t *const out = f.dst + at.batch * f.dst_matrix;
+// Planes of factor[i].alpha * product + factor[i].beta on the diagonal, to their place each.
+__device__ __forceinline__ void power_chunk(const FusedArgs &f, const FusedTile &at, const uint32_t (&v)[32], int c) {
+    const int col = at.col + 32 * c;
+    if (col >= at.cols) return;                    // the same for the whole warp
+    const int diagonal = at.row - col;
+    uint32_t *const patch = reinterpret_cast<uint32_t *>(at.patch);
+#pragma unroll 1
+    for (int i = 0; i < f.outputs; ++i) {
+        const float alpha = f.out[i].alpha, beta = f.out[i].beta;
+        uint16_t *const to = f.out[i].dst + at.batch * f.dst_matrix;
+        uint32_t hi[16], lo[16];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int j0 = c * 32 + h * 16;
-            if (at.col + j0 >= at.cols) return;    // the same for the whole warp; pitches are multiples of 64
-            uint32_t hi[8] = {}, lo[8] = {};
-            if (f.add && live) {
-                load_planes16(add + j0, hi);
-                load_planes16(add + f.add_plane + j0, lo);
+        for (int e = 0; e < 32; e += 2)
+            split_pair(fmaf(alpha, __uint_as_float(v[e]), diagonal == e ? beta : 0.f), fmaf(alpha, __uint_as_float(v[e + 1]), diagonal == e + 1 ? beta : 0.f),
+                       hi[e / 2], lo[e / 2]);
+        if (at.row < at.rows) {
+            uint16_t *const dst = to + at.row * f.dst_pitch + col;
+            store_planes16(dst, hi);
+            store_planes16(dst + f.dst_plane, lo);
+            if (col + 16 < at.cols) {              // (what lies between the last column and the pitch is never read as data)
+                store_planes16(dst + 16, hi + 8);
+                store_planes16(dst + f.dst_plane + 16, lo + 8);
             }
-            float v[16];
+        }
+        if (f.mirror && at.off_diagonal) {
+            // 32 rows become 32 columns: (hi, lo) of an element in a word, turned in the warp's patch, no two lanes in one bank.
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hi[e / 2])), b = __half22float2(*reinterpret_cast<const __half2 *>(&lo[e / 2]));
-                constexpr float down = 1.f / (1 << kHalfLoShift);
-                v[e] = fmaf(f.alpha, __uint_as_float(run[c][h * 16 + e]), f.beta * fmaf(b.x, down, a.x));
-                v[e + 1] = fmaf(f.alpha, __uint_as_float(run[c][h * 16 + e + 1]), f.beta * fmaf(b.y, down, a.y));
+            for (int e = 0; e < 32; e += 2) {
+                patch[at.lane * 32 + (e ^ at.lane)] = __byte_perm(hi[e / 2], lo[e / 2], 0x5410);
+                patch[at.lane * 32 + ((e + 1) ^ at.lane)] = __byte_perm(hi[e / 2], lo[e / 2], 0x7632);
             }
-            if (f.final) {
+            __syncwarp();
+            const int row = at.row - at.lane;      // the first of the warp's rows; all of the result's pitch below
 #pragma unroll
-                for (int e = 0; e < 16; ++e) run[c][h * 16 + e] = __float_as_uint(v[e]);
-                continue;
+            for (int e = 0; e < 32; e += 2) {
+                const uint32_t a = patch[e * 32 + (at.lane ^ e)], b = patch[(e + 1) * 32 + (at.lane ^ (e + 1))];
+                hi[e / 2] = __byte_perm(a, b, 0x5410);
+                lo[e / 2] = __byte_perm(a, b, 0x7632);
             }
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) split_pair(v[e], v[e + 1], hi[e / 2], lo[e / 2]);
-            if (live) {
-                store_planes16(out + at.row * f.dst_pitch + at.col + j0, hi);
-                store_planes16(out + f.dst_plane + at.row * f.dst_pitch + at.col + j0, lo);
-            }
-            if (f.mirror && at.off_diagonal) {
-                // Columns become rows.  Lanes of two neighbouring rows trade one of two columns, so that each writes two elements
-                // of one row of the result: a warp's store covers 64 bytes of each of two rows.
-                const bool odd = at.lane & 1;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t even_col = __byte_perm(hi[e], lo[e], 0x5410), odd_col = __byte_perm(hi[e], lo[e], 0x7632);   // (hi, lo) of a column
-                    const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? even_col : odd_col, 1);
-                    const uint32_t first = odd ? got : even_col, second = odd ? odd_col : got;       // of rows row & ~1 and row | 1
-                    const int col = at.col + j0 + 2 * e + (odd ? 1 : 0), row = at.row & ~1;
-                    if (col < at.cols && row < at.rows) {          // an element past the last row goes into the pitch
-                        uint16_t *const to = out + static_cast<long long>(col) * f.dst_pitch + row;
-                        *reinterpret_cast<uint32_t *>(to) = __byte_perm(first, second, 0x5410);
-                        *reinterpret_cast<uint32_t *>(to + f.dst_plane) = __byte_perm(first, second, 0x7632);
-                    }
+            if (col + at.lane < at.cols && row < at.rows) {
+                uint16_t *const dst = to + static_cast<long long>(col + at.lane) * f.dst_pitch + row;
+                store_planes16(dst, hi);
+                store_planes16(dst + f.dst_plane, lo);
+                if (row + 16 < at.rows) {
+                    store_planes16(dst + 16, hi + 8);
+                    store_planes16(dst + f.dst_plane + 16, lo + 8);
                 }
             }
         }
+    }
 }
 
 }  // namespace

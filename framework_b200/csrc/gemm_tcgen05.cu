@@ -359,6 +359,28 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
         ::"r"(bar), "h"(static_cast<uint16_t>(3))
         : "memory");
 }
+// The same for a pair or a lone CTA.
+template <int CG>
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                         uint32_t accumulate) {
+    if constexpr (CG == 2) {
+        umma_f16_pair(d_tmem, a_lo, a_hi, b_lo, b_hi, idesc, accumulate);
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %2};\n\t"
+            "mov.b64 db, {%3, %4};\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+    if constexpr (CG == 2) umma_commit_pair(bar);
+    else umma_commit(bar);
+}
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -596,21 +618,22 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
     constexpr bool SK = TAIL == kBalanced, CUT = TAIL == kCutTiles;
     constexpr bool HALF = MODE == kHalfThree || MODE == kHalfOne || MODE == kHalfDrain, FAST = MODE != kThreePass;   // FAST: the split warps split nothing
     static_assert(!is_fused(TAIL) || MODE == kHalfDrain, "fused epilogues are built for products of 16-bit halves");
-    static_assert(!HALF || (BN == 256 && BK == 64 && CG == 2 && !TA && !SK), "16-bit halves are built for 256-wide pairs");
+    static_assert(!HALF || (BK == 64 && !TA && !SK && ((BN == 256 && CG == 2) || (BN == 128 && CG == 1 && is_fused(TAIL)))),
+                  "16-bit halves are built for 256-wide pairs, and for lone 128-wide tiles with a fused epilogue");
     constexpr uint32_t ELT = HALF ? 2 : 4;                 // bytes of a staged element
     constexpr int BNL = BN / CG;                           // B rows staged by this CTA
     constexpr uint32_t A_BYTES = BM * BK * ELT;
     constexpr uint32_t B_BYTES = BNL * BK * ELT;
     constexpr uint32_t RAW_BYTES = A_BYTES + B_BYTES;
+    // DRAIN: the large terms are taken out of their accumulator every few k-blocks, while the pipe makes small terms, whose own
+    // chain is as long as the unit (its truncation is 2^-12 of the other's).
+    constexpr bool DRAIN = MODE == kHalfDrain;
     // RUN: a unit's running sum over its pieces takes 128 registers of every epilogue thread, so the warps are laid out in
     // whole warpgroups -- TMA and MMA (and two idle), split, epilogue -- that trade registers.
     // TWO: the large and the small terms of a piece in an accumulator each, all of tensor memory; the epilogue takes both into its
     // registers, whole, before anything is stored, and the next piece begins.
     constexpr bool TWO = MODE == kHalfThree || MODE == kHalfDrain, RUN = TAIL == kRunningSum || TWO;
-    // DRAIN: the large terms are taken out of their accumulator every few k-blocks, while the pipe makes small terms, whose own
-    // chain is as long as the unit (its truncation is 2^-12 of the other's).
-    constexpr bool DRAIN = MODE == kHalfDrain;
-    static_assert(!RUN || (BN == 256 && CG == 2), "running sums are built for 256-wide pairs");
+    static_assert(!RUN || DRAIN || (BN == 256 && CG == 2), "running sums are built for 256-wide pairs");
     constexpr int SPLIT0 = RUN && !TWO ? 4 : 2, EPI0 = SPLIT0 + NS;   // first split and first epilogue warp
     static_assert(!TA || (!FAST && CG == 1 && BK == 32 && NS == 8 && BN <= 128), "unsupported A-from-TMEM variant");
     constexpr uint32_t STAGE_BYTES = FAST ? RAW_BYTES : (TA ? A_BYTES + 2 * B_BYTES : 2 * RAW_BYTES);
@@ -816,7 +839,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        if (cta_rank != 0) mbar_arrive_cta(bar_acc_empty + 8u * slot, 0u);
+                        if (CG == 2 && cta_rank != 0) mbar_arrive_cta(bar_acc_empty + 8u * slot, 0u);
                         else mbar_arrive(bar_acc_empty + 8u * slot);
                     }
                 };
@@ -899,17 +922,34 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                 if (!last_piece) continue;
             }
             if constexpr (is_fused(TAIL)) {
-                const FusedTile at{row0 + lane, q.M, t.tn * BN + chunk_lo * 32, q.N, t.bt, t.tn * 2 + (ew >> 2), t.tm != t.tn, lane};
+                const FusedTile at{row0 + lane, q.M, t.tn * BN + chunk_lo * 32, q.N, t.bt, t.tn * 2 + (ew >> 2), t.tm != t.tn, lane,
+                                   reinterpret_cast<float *>(my_stage)};
+                auto chunks = [&](auto body) {     // one chunk's code for all of them
+#pragma unroll 1
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        body(run[0], c);
+#pragma unroll
+                        for (int d = 1; d < CHUNKS; ++d)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) run[d - 1][e] = run[d][e];
+                    }
+                };
                 if constexpr (TAIL == kRowStats) {
-                    logit_pairs(g.f, at, run, unscale);
+                    PairSum sum;
+                    sum.begin(g.f, at, 32 * CHUNKS);
+                    chunks([&](uint32_t (&v)[32], int c) { sum.chunk(g.f, at, v, c, unscale); });
+                    sum.end(g.f, at);
                     continue;
                 } else if constexpr (TAIL == kRowGrads) {
-                    if (wide) logit_grads<true>(g.f, at, run, unscale);
-                    else logit_grads<false>(g.f, at, run, unscale);
+                    GradRow row;
+                    row.begin(g.f, at, wide);
+                    chunks([&](uint32_t (&v)[32], int c) { grad_chunk(g.f, at, row, v, c, unscale, wide); });
+                    continue;
+                } else if (g.f.outputs > 0) {
+                    if (row0 < q.M) chunks([&](uint32_t (&v)[32], int c) { power_chunk(g.f, at, v, c); });
                     continue;
                 } else {
-                    polynomial(g.f, at, run);
-                    if (!g.f.final) continue;
+                    unscale = g.f.out[0].alpha;
                 }
             }
             if (row0 < q.M) {
@@ -1358,8 +1398,8 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                             if (elect_one()) {
 #pragma unroll
                                 for (int ks = 0; ks < KSTEPS; ++ks)
-                                    umma_f16_pair(d_tmem, ah + ks * a_ks, a_hi, bh + ks * b_ks, b_hi, idesc, ks == 0 ? accumulate : 1u);
-                                if (ends) umma_commit_pair(bar_acc_full);
+                                    umma_f16<CG>(d_tmem, ah + ks * a_ks, a_hi, bh + ks * b_ks, b_hi, idesc, ks == 0 ? accumulate : 1u);
+                                if (ends) commit_to<CG>(bar_acc_full);
                             }
                             __syncwarp();
                         };
@@ -1380,15 +1420,15 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                             if (elect_one()) {
 #pragma unroll
                                 for (int ks = 0; ks < KSTEPS; ++ks) {
-                                    umma_f16_pair(d_tmem + BN, a_lo + ks * a_ks, a_hi, bh + ks * b_ks, b_hi, idesc, ks == 0 ? small_acc : 1u);
-                                    umma_f16_pair(d_tmem + BN, ah + ks * a_ks, a_hi, b_lo + ks * b_ks, b_hi, idesc, 1u);
+                                    umma_f16<CG>(d_tmem + BN, a_lo + ks * a_ks, a_hi, bh + ks * b_ks, b_hi, idesc, ks == 0 ? small_acc : 1u);
+                                    umma_f16<CG>(d_tmem + BN, ah + ks * a_ks, a_hi, b_lo + ks * b_ks, b_hi, idesc, 1u);
                                     if (PLANES == 3 && plane == 1)
-                                        umma_f16_pair(d_tmem + BN, a_lo + ks * a_ks, a_hi, b_lo + ks * b_ks, b_hi, idesc, 1u);
+                                        umma_f16<CG>(d_tmem + BN, a_lo + ks * a_ks, a_hi, b_lo + ks * b_ks, b_hi, idesc, 1u);
                                 }
-                                umma_commit_pair(bar_empty + 8u * stage);
+                                commit_to<CG>(bar_empty + 8u * stage);
                                 if (plane + 1 == PLANES) {
-                                    if (large_first) umma_commit_pair(bar_empty + 8u * hi_stage);
-                                    if (ends && last_piece_of_unit) umma_commit_pair(bar_acc_full + 8u);
+                                    if (large_first) commit_to<CG>(bar_empty + 8u * hi_stage);
+                                    if (ends && last_piece_of_unit) commit_to<CG>(bar_acc_full + 8u);
                                 }
                             }
                             __syncwarp();
@@ -1399,7 +1439,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                         if (!large_first) {
                             large();
                             if (!ok) break;
-                            if (elect_one()) umma_commit_pair(bar_empty + 8u * hi_stage);
+                            if (elect_one()) commit_to<CG>(bar_empty + 8u * hi_stage);
                             __syncwarp();
                         }
                         accumulate = 1u;
@@ -2746,7 +2786,8 @@ static int make_product(const GemmProblem &p, const Plan &pl, bool transposed, i
         // kind::f16: f16 operands, 16-deep k-steps.  K-major rows of 64 elements, one swizzle span (k-step 32 bytes); MN-major chunks
         // of 64 rows, LBO apart, of 64 k-lines in groups of 8 (k-step two groups).
         const uint32_t hi = desc_hi_bits(1024, 2), lbo = static_cast<uint32_t>((pl.bk * 128) >> 4) << 16;
-        k.idesc = (1u << 4) | ((p.ha->k_major ? 0u : 1u) << 15) | ((p.hb->k_major ? 0u : 1u) << 16) | (32u << 17) | (16u << 24);
+        k.idesc = (1u << 4) | ((p.ha->k_major ? 0u : 1u) << 15) | ((p.hb->k_major ? 0u : 1u) << 16) | (static_cast<uint32_t>(pl.bn >> 3) << 17) |
+                  (static_cast<uint32_t>((BM * pl.cg) >> 4) << 24);
         k.a_desc_hi = k.b_desc_hi = hi;
         k.a_desc_lbo = p.ha->k_major ? 0 : lbo;
         k.b_desc_lbo = p.hb->k_major ? 0 : lbo;
@@ -2847,40 +2888,78 @@ int launch_gemm_halves(const GemmProblem *p, int count, float *const *partial, u
     return MNI_B200_OK;
 }
 
+// Tiles of a product with a fused epilogue: 256 x 256 of a pair of CTAs, or 128 x 128 of one where rounds of those take less time.
+// Main loops per contraction element in clocks, and what a round costs beside them (first operands, last stores and what the pipe
+// waits for the epilogue).
+struct FusedTiling {
+    bool lone;
+    int64_t tiles_m, tiles_n, per_batch;
+    long long units, slots;
+};
+static FusedTiling fused_tiling(const GemmProblem &p, bool symmetric, int sm_count) {
+    auto tiling = [&](bool lone) {
+        FusedTiling t;
+        const int64_t side = lone ? 128 : 256;
+        t.lone = lone;
+        t.tiles_m = (p.M + side - 1) / side;
+        t.tiles_n = (p.N + side - 1) / side;
+        t.per_batch = symmetric ? t.tiles_m * (t.tiles_m + 1) / 2 : t.tiles_m * t.tiles_n;
+        t.units = p.batch * t.per_batch;
+        t.slots = lone ? sm_count : std::max(1, sm_count / 2);
+        return t;
+    };
+    const FusedTiling pair = tiling(false), lone = tiling(true);
+    auto clocks = [&](const FusedTiling &t) {
+        const double k = static_cast<double>((p.K + 63) / 64 * 64), rounds = static_cast<double>((t.units + t.slots - 1) / t.slots);
+        return rounds * std::max(t.lone ? 14.0 * k + 800 : 24.4 * k + 800, t.lone ? 4000.0 : 8000.0);
+    };
+    const int env = env_int("MNI_B200_FUSED_LONE", -1);
+    return env == 1 || (env != 0 && clocks(lone) < clocks(pair)) ? lone : pair;
+}
+int fused_stretch(const GemmProblem &p, int sm_count) { return fused_tiling(p, false, sm_count).lone ? 64 : 128; }
+
 // A product from 16-bit planes with one of the fused epilogues: whole tiles, dealt out round-robin.
 int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, bool symmetric, uint32_t *err_word, int sm_count, cudaStream_t stream) {
     if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return MNI_B200_OK;
-    const int64_t tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256;
-    const int64_t per_batch = symmetric ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
-    if (p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.K > 0x7fffffffLL || p.batch * per_batch > 0x3fffffffLL || p.batch * tiles_m * tiles_n > 0x3fffffffLL)
+    const FusedTiling t = fused_tiling(p, symmetric, sm_count);
+    if (p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.K > 0x7fffffffLL || p.batch > 0x7fffffffLL || t.tiles_m * t.tiles_n > 0x3fffffffLL / p.batch)
         return fail(MNI_B200_ERR_TOO_LARGE, "product %lld x %lld x %lld (batch %lld) exceeds the kernels' int32 indexing", (long long)p.M,
                     (long long)p.N, (long long)p.K, (long long)p.batch);
     Plan pl{};
-    pl.bn = 256;
+    pl.bn = t.lone ? 128 : 256;
     pl.bk = 64;
-    pl.cg = 2;
+    pl.cg = t.lone ? 1 : 2;
     pl.patches = 1;
     pl.splits = 1;
     const size_t stage = static_cast<size_t>(BM + 128) * pl.bk * 2, fixed = 1024 + kBarBytes + static_cast<size_t>(kEpiWarps) * kEpiBufBytes;
     pl.stages = static_cast<int>(std::min<size_t>(kMaxStages, (227 * 1024 - fixed) / stage));
     pl.smem = fixed + static_cast<size_t>(pl.stages) * stage;
-    pl.tiles_m = static_cast<int>(tiles_m);
-    pl.tiles_n = static_cast<int>(tiles_n);
-    pl.grid = static_cast<int>(std::min<int64_t>(p.batch * per_batch, std::max(1, sm_count / 2))) * 2;
+    pl.tiles_m = static_cast<int>(t.tiles_m);
+    pl.tiles_n = static_cast<int>(t.tiles_n);
+    pl.grid = static_cast<int>(std::min<long long>(t.units, t.slots)) * pl.cg;
     Product w;
     const int rc = make_product(p, pl, false, p.M, p.N, nullptr, err_word, w);
     if (rc) return rc;
     if (symmetric) {
         w.p.symmetric = 1;
-        w.p.fd_per_batch = make_fastdiv(per_batch);
-        w.p.units = static_cast<int>(p.batch * per_batch);
+        w.p.fd_per_batch = make_fastdiv(t.per_batch);
+        w.p.units = static_cast<int>(t.units);
     }
     const Product *const products[1] = {&w};
     cudaError_t e;
     switch (kind) {
-        case kFusedPairs: e = launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowStats>(pl, products, 1, stream, &f); break;
-        case kFusedGrads: e = launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f); break;
-        default: e = launch_variant<256, 64, kHalfDrain, 2, 2, false, kPolynomial>(pl, products, 1, stream, &f); break;
+        case kFusedPairs:
+            e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kRowStats>(pl, products, 1, stream, &f)
+                       : launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowStats>(pl, products, 1, stream, &f);
+            break;
+        case kFusedGrads:
+            e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kRowGrads>(pl, products, 1, stream, &f)
+                       : launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f);
+            break;
+        default:
+            e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kPolynomial>(pl, products, 1, stream, &f)
+                       : launch_variant<256, 64, kHalfDrain, 2, 2, false, kPolynomial>(pl, products, 1, stream, &f);
+            break;
     }
     if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "gemm_tc_kernel set-up failed: %s", cudaGetErrorString(e));
     MNI_LAUNCH_CHECK("gemm_tc_kernel");

@@ -204,19 +204,23 @@ struct FusedArgs {
     Targets targets;
     int first_class, classes;
     const float *bias;
-    float2 *pairs;                 // [128 columns][row]
+    float2 *pairs;                 // [stretch of columns][row]
     float *at_target;              // [row]
     const float *lse;
     // planes written: [batch][row][pitch], `matrix` and `plane` elements apart
     uint16_t *dst;
     long long dst_pitch, dst_matrix, dst_plane;
-    // polynomial: alpha * product + beta * add, `add` in f16 planes of the result's shape (may be null); final: to the problem's C as f32
-    const uint16_t *add;
-    long long add_pitch, add_matrix, add_plane;
-    float alpha, beta;
-    int final;
+    // powers of matrices: alpha * product + beta on the diagonal, as planes to one or two places (none: as f32 to the problem's C,
+    // times alpha of the first)
+    struct Output {
+        uint16_t *dst;
+        float alpha, beta;
+    } out[2];
+    int outputs;
     int mirror;                    // of a symmetric result: tiles above the diagonal are written below it too
 };
+// Columns that a pair of launch_gemm_fused stands for.
+int fused_stretch(const GemmProblem &p, int sm_count);
 int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, bool symmetric, uint32_t *err_word, int sm_count, cudaStream_t stream);
 constexpr int kGradExponent = 14;      // logit gradients, -1 to 1, are multiplied by 2^14 in f16 planes
 // One line of text naming the kernel variant, tiling, split and grid launch_gemm_tc would use for this problem
