@@ -10,6 +10,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <initializer_list>
 #include <iterator>
@@ -1351,7 +1352,7 @@ int for_planes(Call &c, const mni_b200_view *&v, mni_b200_view &packed) {
 }
 
 // Longest contraction of the large terms in one accumulator of the tensor core, whose adds truncate (7.5e-10 of the sum an element).
-constexpr int kLossChunkK = 512, kMuonChunkK = 128;
+constexpr int kLossChunkK = 512;
 
 // z = x . w of the classes first .. first + count, from planes x (view `xi` of h) and w (view `wi`).
 GemmProblem logits_problem(const LossCall &l, const Halves &h, int wi, int64_t first, int64_t count, HalfOperand &x, HalfOperand &w) {
@@ -1400,7 +1401,7 @@ int loss_fwd_body(Call &c, const LossCall &l, float *loss, float *lse) {
         f.bias = l.bias;
         f.pairs = pairs;
         f.at_target = picked;
-        rc = launch_gemm_fused(p, kFusedPairs, f, false, c.st->err_word, c.gemm_sms(), c.stream);
+        rc = launch_gemm_fused(p, kFusedPairs, f, c.st->err_word, c.gemm_sms(), c.stream);
     } else {
         const size_t z_at = c.arena.reserve(static_cast<size_t>(l.M * l.N) * sizeof(float));
         float *const z = c.dry() ? dry_pointer() : c.at(z_at);
@@ -1528,7 +1529,7 @@ int loss_bwd_planes(Call &c, const LossCall &l, const float *lse, const float *g
             f.dst = static_cast<uint16_t *>(const_cast<void *>(d.ptr));
             f.dst_pitch = d.pitch;
             f.dst_plane = d.plane;
-            rc = launch_gemm_fused(z, kFusedGrads, f, false, c.st->err_word, c.gemm_sms(), c.stream);
+            rc = launch_gemm_fused(z, kFusedGrads, f, c.st->err_word, c.gemm_sms(), c.stream);
             if (rc) return rc;
         }
         GemmProblem p[2];
@@ -1627,82 +1628,40 @@ int step_scales(const NewtonSchulz &ns, std::vector<StepScales> &out) {
     return MNI_B200_OK;
 }
 
-// Steps on `count` matrices of one shape, from planes (x[0] holds the start) to f32 `out` [count][rows][cols].
-struct MuonGroup {
-    int64_t rows, cols, side, count;
-    int64_t x_pitch, x_matrix, s_pitch, s_matrix;          // of x, and of A, R and Q
-    MuonGroup(int64_t r, int64_t c, int64_t n)
-        : rows(r), cols(c), side(std::min(r, c)), count(n), x_pitch(round_up(c, 64)), x_matrix(r * x_pitch), s_pitch(round_up(side, 64)),
-          s_matrix(side * s_pitch) {}
-    size_t x_bytes() const { return static_cast<size_t>(count * x_matrix) * 4; }
-    size_t s_bytes() const { return static_cast<size_t>(count * s_matrix) * 4; }
-};
-int newton_schulz(Call &c, const NewtonSchulz &ns, const std::vector<StepScales> &scales, const MuonGroup &g, uint16_t *const (&x)[2], uint16_t *a,
-                  uint16_t *r, uint16_t *q, float *out) {
-    const bool tall = g.rows > g.cols;
-    auto operand = [&](const uint16_t *p, bool of_x, bool k_major) {
-        HalfOperand o;
-        o.ptr = p;
-        o.k_major = k_major;
-        const int64_t rows = of_x ? g.rows : g.side, cols = of_x ? g.cols : g.side;
-        o.rows = k_major ? rows : cols;
-        o.kdim = k_major ? cols : rows;
-        o.pitch = of_x ? g.x_pitch : g.s_pitch;
-        o.matrix = of_x ? g.x_matrix : g.s_matrix;
-        o.plane = o.matrix * g.count;
-        o.batch = g.count;
-        o.planes = 2;
-        return o;
-    };
-    auto product = [&](const HalfOperand &l, const HalfOperand &r, bool square, std::initializer_list<FusedArgs::Output> outputs, float *final_out) {
-        GemmProblem p;
-        p.M = l.rows; p.N = r.rows; p.K = l.kdim;
-        p.batch = g.count;
-        p.ha = &l; p.hb = &r;
-        p.chunk_k = kMuonChunkK;
-        FusedArgs f{};
-        std::copy(outputs.begin(), outputs.end(), f.out);
-        f.outputs = final_out ? 0 : static_cast<int>(outputs.size());
-        f.dst_pitch = square ? g.s_pitch : g.x_pitch;
-        f.dst_matrix = square ? g.s_matrix : g.x_matrix;
-        f.dst_plane = f.dst_matrix * g.count;
-        f.mirror = square ? 1 : 0;
-        if (final_out) {
-            p.C = final_out;
-            p.ldc = g.cols;
-            p.c_bstride = g.rows * g.cols;
-        }
-        return launch_gemm_fused(p, kFusedPolynomial, f, square, c.st->err_word, c.gemm_sms(), c.stream);
-    };
+// The factors of newton_schulz.cu's planes, from the scales of the matrices they go into.
+std::vector<NewtonStep> step_factors(const NewtonSchulz &ns, const std::vector<StepScales> &scales) {
+    std::vector<NewtonStep> out;
     auto power = [](int e) { return std::ldexp(1.0, e); };
-    for (int k = 0; k < ns.steps; ++k) {
-        const StepScales &e = scales[static_cast<size_t>(k)];
-        const bool last = k + 1 == ns.steps;
-        const int next = last ? 0 : scales[static_cast<size_t>(k) + 1].x;
-        uint16_t *const from = x[k & 1], *const to = x[(k + 1) & 1];
-        // A = x x^T or x^T x (its operands are the same planes), and R = b + c A
-        const HalfOperand xs = operand(from, true, !tall), as = operand(a, false, true), rs = operand(r, false, true), qs = operand(q, false, true);
-        int rc = product(xs, xs, true, {{a, static_cast<float>(power(e.a - 2 * e.x)), 0.f},
-                                        {r, static_cast<float>(ns.c * power(e.r - 2 * e.x)), static_cast<float>(ns.b * power(e.r))}}, nullptr);
-        // Q = a + A R: symmetric, as R is a polynomial in A
-        if (rc == MNI_B200_OK)
-            rc = product(as, rs, true, {{q, static_cast<float>(power(e.q - e.a - e.r)), static_cast<float>(ns.a * power(e.q))}}, nullptr);
-        if (rc) return rc;
-        const FusedArgs::Output out_x{to, static_cast<float>(power(next - e.q - e.x)), 0.f};
-        if (tall) rc = product(operand(from, true, true), qs, false, {out_x}, last ? out : nullptr);      // x Q
-        else rc = product(qs, operand(from, true, false), false, {out_x}, last ? out : nullptr);          // Q x
-        if (rc) return rc;
+    for (size_t k = 0; k < scales.size(); ++k) {
+        const StepScales &e = scales[k];
+        const int next = k + 1 < scales.size() ? scales[k + 1].x : 0;      // the last x is f32
+        out.push_back(NewtonStep{static_cast<float>(power(e.a - 2 * e.x)), static_cast<float>(ns.c * power(e.r - 2 * e.x)),
+                                 static_cast<float>(ns.b * power(e.r)), static_cast<float>(power(e.q - e.a - e.r)),
+                                 static_cast<float>(ns.a * power(e.q)), static_cast<float>(power(next - e.q - e.x))});
     }
-    return MNI_B200_OK;
+    return out;
 }
 
-// Scratch that the matrices which are worked on at a time may take: enough to fill the GPU many times over.
-constexpr size_t kMuonScratch = size_t{1} << 30;
+// Scratch that the matrices of one launch may take: enough to fill the GPU many times over.
+constexpr size_t kMuonScratch = size_t{2} << 30;
 
-// The entries are `e`; where an entry has a parameter it is updated, otherwise the result goes to e[i].x (matrix after matrix).
+// The entries are `e`; where an entry has a parameter it is updated, otherwise the result goes to e[i].x.
 int muon_body(Call &c, const std::vector<MuonEntry> &e, const NewtonSchulz &ns, const std::vector<StepScales> &scales, float mu, bool nesterov, float eps,
               float decay) {
-    // matrices of one shape, in the order of their first
+    const bool update = e[0].param != nullptr;
+    if (ns.steps == 0) {                           // the normalised update itself
+        std::vector<MuonEntry> all = e;
+        const size_t sums = c.arena.reserve(muon_partial_bytes(all.data(), static_cast<int64_t>(all.size())));
+        for (MuonEntry &m : all) {
+            const size_t at = update ? c.arena.reserve(static_cast<size_t>(m.n) * 4) : 0;
+            if (update && !c.dry()) m.x = c.at(at);
+        }
+        if (c.dry()) return MNI_B200_OK;
+        const int rc = launch_muon_start(all.data(), static_cast<int64_t>(all.size()), mu, nesterov, eps, reinterpret_cast<double *>(c.at(sums)), 0, nullptr, 0,
+                                         c.stream);
+        return rc || !update ? rc : launch_muon_update(all.data(), static_cast<int64_t>(all.size()), decay, c.stream);
+    }
+    // matrices of one shape together, in the order of their first
     std::map<std::pair<int64_t, int64_t>, size_t> index;
     std::vector<std::vector<MuonEntry>> groups;
     for (const MuonEntry &m : e) {
@@ -1710,40 +1669,68 @@ int muon_body(Call &c, const std::vector<MuonEntry> &e, const NewtonSchulz &ns, 
         if (found.second) groups.emplace_back();
         groups[found.first->second].push_back(m);
     }
-    for (std::vector<MuonEntry> &all : groups) {
-        const MuonGroup one(all[0].rows, all[0].cols, 1);
-        const bool update = all[0].param != nullptr;
-        if (one.x_matrix / 8 > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "a matrix of %lld x %lld is too large", (long long)one.rows, (long long)one.cols);
-        const size_t each = 2 * one.x_bytes() + 3 * one.s_bytes() + (update ? static_cast<size_t>(one.rows * one.cols) * 4 : 0);
-        const int64_t at_once = std::max<int64_t>(1, std::min<int64_t>(65535, static_cast<int64_t>(kMuonScratch / each)));
-        for (size_t first = 0; first < all.size(); first += static_cast<size_t>(at_once)) {
-            const int64_t count = std::min<int64_t>(at_once, static_cast<int64_t>(all.size() - first));
-            MuonEntry *const part = all.data() + first;
-            const MuonGroup g(one.rows, one.cols, count);
-            const size_t mark = c.arena.used;
-            const size_t sums = c.arena.reserve(muon_partial_bytes(part, count)), x0 = c.arena.reserve(g.x_bytes()), x1 = c.arena.reserve(g.x_bytes()),
-                         a = c.arena.reserve(g.s_bytes()), r = c.arena.reserve(g.s_bytes()), q = c.arena.reserve(g.s_bytes()),
-                         result = update ? c.arena.reserve(static_cast<size_t>(count * g.rows * g.cols) * 4) : 0;
-            c.arena.used = mark;
-            if (c.dry()) continue;
-            if (update)
-                for (int64_t i = 0; i < count; ++i) part[i].x = c.at(result) + i * g.rows * g.cols;
-            MuonPlanes planes;
-            if (ns.steps > 0) {
-                planes.dst = reinterpret_cast<uint16_t *>(c.at(x0));
-                planes.pitch = g.x_pitch;
-                planes.matrix = g.x_matrix;
-                planes.plane = g.x_matrix * count;
-                planes.exponent = scales[0].x;
+    const std::vector<NewtonStep> factors = step_factors(ns, scales);
+    size_t group = 0, at = 0;                      // the next matrix
+    while (group < groups.size()) {
+        const size_t mark = c.arena.used;
+        std::vector<MuonEntry> list;
+        std::vector<NewtonProblem> problems;
+        std::vector<std::array<size_t, 5>> places;
+        size_t bytes = 0;
+        while (group < groups.size() && problems.size() < kNewtonGroups && list.size() < kNewtonMatrices) {
+            const std::vector<MuonEntry> &all = groups[group];
+            NewtonProblem n{};
+            n.rows = all[0].rows;
+            n.cols = all[0].cols;
+            n.x_pitch = round_up(n.cols, 64);
+            n.s_pitch = round_up(n.side(), 64);
+            const int64_t x_matrix = n.rows * n.x_pitch, s_matrix = n.side() * n.s_pitch;
+            if (x_matrix / 8 > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "a matrix of %lld x %lld is too large", (long long)n.rows, (long long)n.cols);
+            const size_t each = static_cast<size_t>(2 * x_matrix + 3 * s_matrix) * 4;
+            const size_t room = bytes < kMuonScratch ? (kMuonScratch - bytes) / each : 0;
+            const size_t take = std::min({std::max<size_t>(room, problems.empty() ? 1 : 0), all.size() - at, kNewtonMatrices - list.size()});
+            if (take == 0) break;
+            n.count = static_cast<int64_t>(take);
+            bytes += take * each;
+            list.insert(list.end(), all.begin() + static_cast<std::ptrdiff_t>(at), all.begin() + static_cast<std::ptrdiff_t>(at + take));
+            std::array<size_t, 5> place;
+            for (int k = 0; k < 5; ++k) place[static_cast<size_t>(k)] = c.arena.reserve(take * static_cast<size_t>(k < 2 ? x_matrix : s_matrix) * 4);
+            places.push_back(place);
+            problems.push_back(n);
+            at += take;
+            if (at == all.size()) {
+                ++group;
+                at = 0;
             }
-            int rc = launch_muon_start(part, count, mu, nesterov, eps, reinterpret_cast<double *>(c.at(sums)), planes, c.stream);
-            uint16_t *const x[2] = {reinterpret_cast<uint16_t *>(c.at(x0)), reinterpret_cast<uint16_t *>(c.at(x1))};
-            if (rc == MNI_B200_OK)
-                rc = newton_schulz(c, ns, scales, g, x, reinterpret_cast<uint16_t *>(c.at(a)), reinterpret_cast<uint16_t *>(c.at(r)),
-                                   reinterpret_cast<uint16_t *>(c.at(q)), part[0].x);
-            if (rc == MNI_B200_OK && update) rc = launch_muon_update(part, count, decay, c.stream);
-            if (rc) return rc;
         }
+        const int words = 1 + 3 * static_cast<int>(list.size());
+        const size_t sums = c.arena.reserve(muon_partial_bytes(list.data(), static_cast<int64_t>(list.size())));
+        const size_t counters = c.arena.reserve(static_cast<size_t>(words) * sizeof(unsigned));
+        c.arena.used = mark;
+        if (c.dry()) continue;
+        std::vector<float *> out;
+        std::vector<float> scale;
+        size_t m = 0;
+        for (size_t i = 0; i < problems.size(); ++i) {
+            NewtonProblem &n = problems[i];
+            uint16_t **const to[5] = {&n.x[0], &n.x[1], &n.a, &n.r, &n.q};
+            for (int k = 0; k < 5; ++k) *to[k] = reinterpret_cast<uint16_t *>(c.at(places[i][static_cast<size_t>(k)]));
+            for (int64_t k = 0; k < n.count; ++k, ++m) {
+                MuonEntry &entry = list[m];
+                entry.planes = n.x[0] + k * n.rows * n.x_pitch;
+                entry.pitch = n.x_pitch;
+                entry.plane = n.rows * n.x_pitch * n.count;
+                out.push_back(update ? entry.param : entry.x);
+                scale.push_back(entry.scale);
+            }
+        }
+        unsigned *const words_at = reinterpret_cast<unsigned *>(c.at(counters));
+        int rc = launch_muon_start(list.data(), static_cast<int64_t>(list.size()), mu, nesterov, eps, reinterpret_cast<double *>(c.at(sums)), scales[0].x,
+                                   words_at, words, c.stream);
+        if (rc == MNI_B200_OK)
+            rc = launch_newton_schulz(problems.data(), static_cast<int>(problems.size()), factors.data(), ns.steps, out.data(), scale.data(), update, decay,
+                                      words_at, c.st->err_word, c.gemm_sms(), c.stream);
+        if (rc) return rc;
     }
     return MNI_B200_OK;
 }
@@ -2163,7 +2150,7 @@ int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float 
         }
         std::vector<MuonEntry> e;
         for (int64_t i = 0; i < batch; ++i)
-            e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, rows, cols, rows * cols, 0.f});
+            e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, nullptr, 0, 0, rows, cols, rows * cols, 0.f});
         return muon_body(call, e, ns, scales, 0.f, false, eps, 1.f);
     });
 }
@@ -2186,7 +2173,7 @@ int mni_b200_muon_step(int64_t count, float *const *params, float *const *moment
         if (!params[i] || !momenta[i] || !grads[i]) return fail(MNI_B200_ERR_ARG, "null pointer");
         if (share_memory(params[i], momenta[i], n) || share_memory(params[i], grads[i], n) || share_memory(momenta[i], grads[i], n))
             return fail(MNI_B200_ERR_ARG, "entry %lld: param, momentum and grad share memory", (long long)i);
-        e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, rows[i], cols[i], n, lr * scales[i]});
+        e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, nullptr, 0, 0, rows[i], cols[i], n, lr * scales[i]});
     }
     // Entries that share memory with one before them begin another round, which starts from what that one left.
     for (size_t first = 0; first < e.size();) {

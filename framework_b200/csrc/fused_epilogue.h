@@ -178,8 +178,16 @@ __device__ __forceinline__ void grad_chunk(const FusedArgs &f, const FusedTile &
     store_planes16(dst + f.dst_plane + 16, lo + 8);
 }
 
-// Planes of factor[i].alpha * product + factor[i].beta on the diagonal, to their place each.
-__device__ __forceinline__ void power_chunk(const FusedArgs &f, const FusedTile &at, const uint32_t (&v)[32], int c) {
+// Planes of alpha * product + beta on the diagonal, to one or two places.
+struct PowerOutputs {
+    long long dst_pitch, dst_matrix, dst_plane;
+    struct {
+        uint16_t *dst;
+        float alpha, beta;
+    } out[2];
+    int outputs;
+};
+__device__ __forceinline__ void power_chunk(const PowerOutputs &f, const FusedTile &at, const uint32_t (&v)[32], int c) {
     const int col = at.col + 32 * c;
     if (col >= at.cols) return;                    // the same for the whole warp
     const int diagonal = at.row - col;
@@ -202,7 +210,7 @@ __device__ __forceinline__ void power_chunk(const FusedArgs &f, const FusedTile 
                 store_planes16(dst + f.dst_plane + 16, lo + 8);
             }
         }
-        if (f.mirror && at.off_diagonal) {
+        if (at.off_diagonal) {
             // 32 rows become 32 columns: (hi, lo) of an element in a word, turned in the warp's patch, no two lanes in one bank.
             __syncwarp();
 #pragma unroll

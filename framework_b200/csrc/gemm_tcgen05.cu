@@ -44,8 +44,8 @@
 //               epilogue's registers every chunk_k elements.  Their chain is that long and no longer (the small terms', whose truncation is
 //               2^-12 of it, is the unit), and the pipe, which has small terms to make meanwhile, does not wait.
 //
-// Three epilogues of kHalfDrain keep a product out of memory altogether (fused_epilogue.h): the pairs (maximum, sum of exponentials) of
-// logits, the gradient of logits as planes for the products that follow, and a polynomial in a matrix, planes again.
+// Two epilogues of kHalfDrain keep a product out of memory altogether (fused_epilogue.h): the pairs (maximum, sum of exponentials) of
+// logits, and the gradient of logits as planes for the products that follow.
 //
 // CG = 2: two CTAs of a cluster share a 256 x BN tile (cta_group::2 MMAs issued by the leader).
 // Work is dealt out as whole tiles, round-robin over the CTAs (pairs).  The tiles of a badly ragged wave are cut into
@@ -65,6 +65,7 @@
 #include "activation.h"
 #include "fused_epilogue.h"
 #include "internal.h"
+#include "tcgen05.h"
 
 #include <stdio.h>
 #include <string.h>
@@ -85,11 +86,10 @@ constexpr int kSkMaxShare = 6;                             // balanced tail: mos
 constexpr int kEpiWarps = 8;                                // two per TMEM lane quarter, half of the columns each
 constexpr int kEpiBufBytes = 32 * 128;                     // one 32 x 32 f32 patch
 constexpr int kBarBytes = (3 * kMaxStages + 4) * 8 + 16;
-constexpr long long kWaitCycles = 4000000000LL;            // default limit of every device-side wait: ~2 s at 2 GHz
 
 enum OperandMode { kKMajor = 0, kMnMultiBox = 1, kMnSingleBox = 2 };
-enum TailMode { kWholeTiles = 0, kBalanced = 1, kCutTiles = 2, kRunningSum = 3, kRowStats = 4, kRowGrads = 5, kPolynomial = 6 };
-// The last three: whole tiles of kHalfDrain with an epilogue of their own.
+enum TailMode { kWholeTiles = 0, kBalanced = 1, kCutTiles = 2, kRunningSum = 3, kRowStats = 4, kRowGrads = 5 };
+// The last two: whole tiles of kHalfDrain with an epilogue of their own.
 __host__ __device__ constexpr bool is_fused(int tail) { return tail >= kRowStats; }
 // How a product is computed: operands as f32 (three TF32 passes, or one), or as the 16-bit halves that split_half_kernel has made
 // of them (three passes, or one).
@@ -147,7 +147,6 @@ struct KParams {
     // 16-bit halves: what split_half_kernel left beside them
     const int *a_exp, *b_exp;              // the operands were multiplied by 2^exponent
     const unsigned int *half_status;       // bit 0: some operand's range did not fit
-    int symmetric;                         // kPolynomial: only tiles on and above the diagonal are computed
 };
 
 // What a launch computes: one product, or (16-bit planes) two that need nothing from each other, the units of the second dealt
@@ -166,252 +165,6 @@ struct FusedProduct {
     int count;
     FusedArgs f;
 };
-
-// ------------------------------------------------------------------ PTX helpers
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok;
-}
-// Bounded wait.  Returns false if the CTA is aborting (this waiter or another gave up).
-// With `timed`, `waited` accumulates the cycles spent blocked (role-level wait accounting, including
-// the time the first try_wait is suspended by the hardware); without it the satisfied case costs one
-// try_wait and no clock reads.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag,
-                                          unsigned int *err, uint32_t code, long long &waited, bool timed,
-                                          long long limit) {
-    long long t0 = 0;
-    if (timed) t0 = clock64();
-    if (mbar_try_wait(bar, parity)) {
-        if (timed) waited += clock64() - t0;
-        return true;
-    }
-    if (!timed) t0 = clock64();
-    uint32_t spins = 0;
-    while (true) {
-        if (mbar_try_wait(bar, parity)) {
-            if (timed) waited += clock64() - t0;
-            return true;
-        }
-        if ((++spins & 63u) == 0u) {
-            if (*abort_flag) return false;
-            if (clock64() - t0 > limit) {
-                *abort_flag = 1u;
-                atomicCAS(err, 0u, code);
-                return false;
-            }
-        }
-    }
-}
-// Warp-collective form: every lane polls, the verdict is made uniform.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag,
-                                               unsigned int *err, uint32_t code, long long &waited, bool timed,
-                                               long long limit) {
-    const bool ok = mbar_wait(bar, parity, abort_flag, err, code, waited, timed, limit);
-    return __all_sync(0xffffffffu, ok);
-}
-// Non-blocking look at a barrier phase (try_wait may suspend the thread; this never does).
-__device__ __forceinline__ uint32_t mbar_test_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok;
-}
-// True in exactly one lane of a converged warp.  The TMA and MMA issuing warps run their loops
-// warp-uniformly and predicate only the issuing instruction with this: descriptors and
-// coordinates then stay in uniform registers, which makes an MMA issue ~3x cheaper than from a
-// single-lane branch (measured: 40 vs 120 cycles).
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile(
-        "{\n\t.reg .b32 rx;\n\t.reg .pred px;\n\t"
-        "elect.sync rx|px, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, px;\n\t}"
-        : "=r"(pred));
-    return pred != 0;
-}
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0,
-                                            int c1, int c2, int c3, int c4) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
-        "r"(c4)
-        : "memory");
-}
-__device__ __forceinline__ void tma_store_5d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
-    asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(0), "r"(0)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_reduce_add_5d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
-    asm volatile(
-        "cp.reduce.async.bulk.tensor.5d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
-        ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(0), "r"(0)
-        : "memory");
-}
-__device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                          uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %5, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// A operand from tensor memory (lanes = rows, one 32-bit column per k element), B from shared memory.
-__device__ __forceinline__ void umma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi,
-                                             uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "setp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
-}
-// ---- CTA-pair (cta_group::2) forms: one MMA spans two SMs; the leader CTA issues it.
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Arrive on the barrier at the same shared-memory offset in CTA `cta` of the cluster.
-__device__ __forceinline__ void mbar_arrive_cta(uint32_t bar, uint32_t cta) {
-    asm volatile(
-        "{\n\t.reg .b32 ra;\n\t"
-        "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
-        "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}"
-        ::"r"(bar), "r"(cta)
-        : "memory");
-}
-__device__ __forceinline__ void umma_tf32_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                               uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::tf32 [%0], da, db, %5, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                              uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// Commit that arrives on the barrier at this offset in both CTAs of the pair.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-        ::"r"(bar), "h"(static_cast<uint16_t>(3))
-        : "memory");
-}
-// The same for a pair or a lone CTA.
-template <int CG>
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                         uint32_t accumulate) {
-    if constexpr (CG == 2) {
-        umma_f16_pair(d_tmem, a_lo, a_hi, b_lo, b_hi, idesc, accumulate);
-    } else {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-            "mov.b64 da, {%1, %2};\n\t"
-            "mov.b64 db, {%3, %4};\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}"
-            ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-            : "memory");
-    }
-}
-template <int CG>
-__device__ __forceinline__ void commit_to(uint32_t bar) {
-    if constexpr (CG == 2) umma_commit_pair(bar);
-    else umma_commit(bar);
-}
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
-          "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
-          "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
-          "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 
 struct TileCoord {
     int bt, tm, tn, split, it0, it1;
@@ -441,22 +194,8 @@ __device__ __forceinline__ TileCoord decode_unit(const KParams &p, int unit) {
     t.park = 0;
     t.chunk = 0;
     t.tile = tile;
-    t.bt = fd_div(tile, p.fd_per_batch);
-    if constexpr (TAIL == kPolynomial) {
-        if (p.symmetric) {                         // row tm of the triangle begins at tm * (2T + 1 - tm) / 2
-            const int r = tile - t.bt * static_cast<int>(p.fd_per_batch.d), n = p.tiles_m, b = 2 * n + 1;
-            int tm = static_cast<int>((b - sqrtf(static_cast<float>(b) * b - 8.f * r)) * 0.5f);
-            tm = max(0, min(n - 1, tm));
-            while (tm > 0 && tm * (b - tm) / 2 > r) --tm;
-            while (tm + 1 < n && (tm + 1) * (b - tm - 1) / 2 <= r) ++tm;
-            t.tm = tm;
-            t.tn = tm + (r - tm * (b - tm) / 2);
-            t.it0 = 0;
-            t.it1 = p.fold * p.kiters;
-            return t;
-        }
-    }
     const int per_batch = p.tiles_m * p.tiles_n;
+    t.bt = fd_div(tile, p.fd_per_batch);
     const int r = tile - t.bt * per_batch;
     const int group_sz = p.group_m * p.tiles_n;
     const int g = fd_div(r, p.fd_group_sz);
@@ -718,7 +457,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
     if (p.dep_mode == 1 && threadIdx.x == 0) grid_dependency_trigger();
     // HALF: wide if some operand's range did not fit f16, and the planes hold bf16 thirds, unscaled.
     bool wide = false, huge = false;
-    if constexpr (HALF && TAIL != kPolynomial) {       // (its planes are f16 always)
+    if constexpr (HALF) {
         const unsigned int status = __ldcg(p.half_status);
         wide = (status & 1u) != 0;
         huge = (status & 2u) != 0;
@@ -752,7 +491,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
         const Product &w = g.s[HALF ? prod : 0];
         const KParams &q = HALF ? w.p : p;
         float unscale = 1.f;
-        if constexpr (HALF && TAIL != kPolynomial) {
+        if constexpr (HALF) {
             int ea = __ldcg(q.a_exp), eb = __ldcg(q.b_exp);          // at most 60 either way
             if (wide) { ea = half_wide_exponent(ea, huge); eb = half_wide_exponent(eb, huge); }
             unscale = __uint_as_float(static_cast<uint32_t>(127 - ea - eb) << 23);
@@ -939,18 +678,12 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                     sum.begin(g.f, at, 32 * CHUNKS);
                     chunks([&](uint32_t (&v)[32], int c) { sum.chunk(g.f, at, v, c, unscale); });
                     sum.end(g.f, at);
-                    continue;
-                } else if constexpr (TAIL == kRowGrads) {
+                } else {
                     GradRow row;
                     row.begin(g.f, at, wide);
                     chunks([&](uint32_t (&v)[32], int c) { grad_chunk(g.f, at, row, v, c, unscale, wide); });
-                    continue;
-                } else if (g.f.outputs > 0) {
-                    if (row0 < q.M) chunks([&](uint32_t (&v)[32], int c) { power_chunk(g.f, at, v, c); });
-                    continue;
-                } else {
-                    unscale = g.f.out[0].alpha;
                 }
+                continue;
             }
             if (row0 < q.M) {
 #pragma unroll(RUN ? CHUNKS : 1)
@@ -2023,10 +1756,10 @@ int make_operand_map(CUtensorMap *map, const Operand &op, int box_rows, int bk, 
 
 // Tensor map of an operand in 16-bit halves.  K-major: (kdim, rows, batch, plane) in boxes of 64 x 128.  MN-major: (64 contiguous
 // rows, kdim, chunks of 64 rows, batch, plane) in boxes of 64 x 64 x 2; the pitch is a multiple of 64 there.
-int make_half_map(CUtensorMap *map, const HalfOperand &op, int *mode) {
+int make_half_map(CUtensorMap *map, const HalfOperand &op, int *mode, int box_rows = 128) {
     if (!encode_fn()) return fail(MNI_B200_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
     cuuint64_t dims[5], strides[4];
-    cuuint32_t box[5] = {64, 128, 1, 1, 1};
+    cuuint32_t box[5] = {64, static_cast<cuuint32_t>(box_rows), 1, 1, 1};
     const cuuint64_t pitch = static_cast<cuuint64_t>(op.pitch) * 2, matrix = static_cast<cuuint64_t>(op.matrix) * 2,
                      plane = static_cast<cuuint64_t>(op.plane) * 2, batch = static_cast<cuuint64_t>(op.batch);
     if (op.k_major) {
@@ -2036,7 +1769,7 @@ int make_half_map(CUtensorMap *map, const HalfOperand &op, int *mode) {
     } else {
         dims[0] = 64; dims[1] = static_cast<cuuint64_t>(op.kdim); dims[2] = static_cast<cuuint64_t>((op.rows + 63) / 64); dims[3] = batch; dims[4] = static_cast<cuuint64_t>(op.planes);
         strides[0] = pitch; strides[1] = 128; strides[2] = matrix; strides[3] = plane;
-        box[1] = 64; box[2] = 2;
+        box[1] = 64; box[2] = static_cast<cuuint32_t>(box_rows / 64);
         *mode = kMnSingleBox;
     }
     const CUresult r = encode(map, op.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
@@ -2542,6 +2275,11 @@ static bool can_fuse_activation(const GemmProblem &p, const Plan &pl) {
 
 bool gemm_tc_can_fuse_activation(const GemmProblem &p, int sm_count) { return can_fuse_activation(p, make_plan(p, sm_count)); }
 
+int half_operand_map(CUtensorMap *map, const HalfOperand &op, int box_rows) {
+    int mode;
+    return make_half_map(map, op, &mode, box_rows);
+}
+
 static int64_t partial_pitch(int64_t n) { return (n + 3) / 4 * 4; }
 
 static size_t partial_bytes(const GemmProblem &p, const Plan &pl, int64_t out_rows, int64_t out_cols);
@@ -2893,18 +2631,17 @@ int launch_gemm_halves(const GemmProblem *p, int count, float *const *partial, u
 // waits for the epilogue).
 struct FusedTiling {
     bool lone;
-    int64_t tiles_m, tiles_n, per_batch;
+    int64_t tiles_m, tiles_n;
     long long units, slots;
 };
-static FusedTiling fused_tiling(const GemmProblem &p, bool symmetric, int sm_count) {
+static FusedTiling fused_tiling(const GemmProblem &p, int sm_count) {
     auto tiling = [&](bool lone) {
         FusedTiling t;
         const int64_t side = lone ? 128 : 256;
         t.lone = lone;
         t.tiles_m = (p.M + side - 1) / side;
         t.tiles_n = (p.N + side - 1) / side;
-        t.per_batch = symmetric ? t.tiles_m * (t.tiles_m + 1) / 2 : t.tiles_m * t.tiles_n;
-        t.units = p.batch * t.per_batch;
+        t.units = p.batch * t.tiles_m * t.tiles_n;
         t.slots = lone ? sm_count : std::max(1, sm_count / 2);
         return t;
     };
@@ -2916,12 +2653,12 @@ static FusedTiling fused_tiling(const GemmProblem &p, bool symmetric, int sm_cou
     const int env = env_int("MNI_B200_FUSED_LONE", -1);
     return env == 1 || (env != 0 && clocks(lone) < clocks(pair)) ? lone : pair;
 }
-int fused_stretch(const GemmProblem &p, int sm_count) { return fused_tiling(p, false, sm_count).lone ? 64 : 128; }
+int fused_stretch(const GemmProblem &p, int sm_count) { return fused_tiling(p, sm_count).lone ? 64 : 128; }
 
 // A product from 16-bit planes with one of the fused epilogues: whole tiles, dealt out round-robin.
-int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, bool symmetric, uint32_t *err_word, int sm_count, cudaStream_t stream) {
+int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, uint32_t *err_word, int sm_count, cudaStream_t stream) {
     if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return MNI_B200_OK;
-    const FusedTiling t = fused_tiling(p, symmetric, sm_count);
+    const FusedTiling t = fused_tiling(p, sm_count);
     if (p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.K > 0x7fffffffLL || p.batch > 0x7fffffffLL || t.tiles_m * t.tiles_n > 0x3fffffffLL / p.batch)
         return fail(MNI_B200_ERR_TOO_LARGE, "product %lld x %lld x %lld (batch %lld) exceeds the kernels' int32 indexing", (long long)p.M,
                     (long long)p.N, (long long)p.K, (long long)p.batch);
@@ -2940,27 +2677,14 @@ int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, 
     Product w;
     const int rc = make_product(p, pl, false, p.M, p.N, nullptr, err_word, w);
     if (rc) return rc;
-    if (symmetric) {
-        w.p.symmetric = 1;
-        w.p.fd_per_batch = make_fastdiv(t.per_batch);
-        w.p.units = static_cast<int>(t.units);
-    }
     const Product *const products[1] = {&w};
     cudaError_t e;
-    switch (kind) {
-        case kFusedPairs:
-            e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kRowStats>(pl, products, 1, stream, &f)
-                       : launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowStats>(pl, products, 1, stream, &f);
-            break;
-        case kFusedGrads:
-            e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kRowGrads>(pl, products, 1, stream, &f)
-                       : launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f);
-            break;
-        default:
-            e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kPolynomial>(pl, products, 1, stream, &f)
-                       : launch_variant<256, 64, kHalfDrain, 2, 2, false, kPolynomial>(pl, products, 1, stream, &f);
-            break;
-    }
+    if (kind == kFusedPairs)
+        e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kRowStats>(pl, products, 1, stream, &f)
+                   : launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowStats>(pl, products, 1, stream, &f);
+    else
+        e = t.lone ? launch_variant<128, 64, kHalfDrain, 2, 1, false, kRowGrads>(pl, products, 1, stream, &f)
+                   : launch_variant<256, 64, kHalfDrain, 2, 2, false, kRowGrads>(pl, products, 1, stream, &f);
     if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "gemm_tc_kernel set-up failed: %s", cudaGetErrorString(e));
     MNI_LAUNCH_CHECK("gemm_tc_kernel");
     return MNI_B200_OK;

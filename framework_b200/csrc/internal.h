@@ -138,6 +138,9 @@ struct HalfOperand {
 };
 // lo = (x - hi) * 2^kHalfLoShift: the whole range of f16 serves the part below hi's last bit
 constexpr int kHalfLoShift = 12;
+// Tensor map of an operand in planes: boxes of 64 contraction elements by box_rows (64 or 128), swizzled; coordinates (k, row, batch,
+// plane, 0), or for an MN-major one (0, k, row / 64, batch, plane).
+int half_operand_map(CUtensorMap *map, const HalfOperand &op, int box_rows);
 // f16 planes: exponents lie within this either way.
 constexpr int kHalfMaxExp = 60;
 // The exponent of bf16 planes, from that of f16 ones.  Numbers so small that their parts would run into bf16's smallest are
@@ -194,7 +197,7 @@ double gemm_halves_estimate_us(const GemmProblem *p, int count, int sm_count);  
 void gemm_halves_describe(const GemmProblem *p, int count, int sm_count, std::string *lines);
 
 // Products from 16-bit planes whose results leave the kernel in another form (fused_epilogue.h).
-enum FusedKind { kFusedPairs, kFusedGrads, kFusedPolynomial };
+enum FusedKind { kFusedPairs, kFusedGrads };
 struct Targets {
     const void *ptr;               // whole numbers of `bytes` bytes (4 or 8), one per row; below zero: the row is left out
     int bytes;
@@ -210,18 +213,10 @@ struct FusedArgs {
     // planes written: [batch][row][pitch], `matrix` and `plane` elements apart
     uint16_t *dst;
     long long dst_pitch, dst_matrix, dst_plane;
-    // powers of matrices: alpha * product + beta on the diagonal, as planes to one or two places (none: as f32 to the problem's C,
-    // times alpha of the first)
-    struct Output {
-        uint16_t *dst;
-        float alpha, beta;
-    } out[2];
-    int outputs;
-    int mirror;                    // of a symmetric result: tiles above the diagonal are written below it too
 };
 // Columns that a pair of launch_gemm_fused stands for.
 int fused_stretch(const GemmProblem &p, int sm_count);
-int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, bool symmetric, uint32_t *err_word, int sm_count, cudaStream_t stream);
+int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, uint32_t *err_word, int sm_count, cudaStream_t stream);
 constexpr int kGradExponent = 14;      // logit gradients, -1 to 1, are multiplied by 2^14 in f16 planes
 // One line of text naming the kernel variant, tiling, split and grid launch_gemm_tc would use for this problem
 // on a device with `sm_count` SMs.  Pure host arithmetic: touches no device.
@@ -382,25 +377,37 @@ int launch_grad_column_sums(const uint16_t *planes, int64_t pitch, int64_t plane
 // z -> weights * (exp(z - lse) - [class = target])
 int launch_logit_grad(float *z, int64_t rows, int64_t n, const Targets &targets, const float *lse, const float *weights, cudaStream_t stream);
 
-// Newton-Schulz updates (muon.cu).
+// Newton-Schulz updates (muon.cu, newton_schulz.cu).
 struct MuonEntry {
     float *param, *momentum;       // null for a matrix that is only made orthogonal
     const float *grad;
-    float *x;                      // the normalised update, then the orthogonal matrix
+    float *x;                      // the normalised update in f32, or
+    uint16_t *planes;              // ... in f16 planes, rows of `pitch`, the second `plane` elements behind the first
+    int64_t pitch, plane;
     int64_t rows, cols, n;
     float scale;                   // of the update (learning rate included)
 };
 // momentum = mu * momentum + grad, and the sums of squares of the update u = grad + mu * momentum (nesterov) or momentum, or
-// grad where there is no momentum; then x = u / (norm + eps)
+// grad where there is no momentum; then u / (norm + eps) into every entry's x, or planes times 2^exponent.  Also zeroes `words` counters.
 size_t muon_partial_bytes(const MuonEntry *e, int64_t count);
-// Where x goes: f16 planes times 2^exponent, matrix after matrix, or (dst null) to each entry's x in f32.
-struct MuonPlanes {
-    uint16_t *dst = nullptr;
-    int64_t pitch = 0, matrix = 0, plane = 0;
-    int exponent = 0;
+int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, int exponent, unsigned *counters,
+                      int words, cudaStream_t stream);
+// `count` matrices of one shape in planes, one behind the other: x[0] holds the start; x[1], a, r, q are scratch.
+struct NewtonProblem {
+    int64_t rows, cols, count;
+    uint16_t *x[2], *a, *r, *q;
+    int64_t x_pitch, s_pitch;      // of x, and of the square matrices
+    int64_t side() const { return rows < cols ? rows : cols; }
+    bool tall() const { return rows > cols; }
 };
-int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, const MuonPlanes &planes,
-                      cudaStream_t stream);
+// Factors of a step's planes: of x x^T in A, of x x^T and the identity in R, of A R and the identity in Q, of Q x in the next x.
+struct NewtonStep {
+    float a, r, r_diagonal, q, q_diagonal, x;
+};
+constexpr int kNewtonGroups = 12, kNewtonMatrices = 512, kNewtonSteps = 100;      // of a launch (25 KB of kernel parameters)
+// out[i] = x of matrix i, or (update) decay * out[i] - scale[i] * x.  counters: 1 + 3 * matrices words, zero.
+int launch_newton_schulz(const NewtonProblem *problems, int count, const NewtonStep *steps, int step_count, float *const *out, const float *scale, bool update,
+                         float decay, unsigned *counters, uint32_t *err_word, int sm_count, cudaStream_t stream);
 // param = decay * param - scale * x
 int launch_muon_update(const MuonEntry *e, int64_t count, float decay, cudaStream_t stream);
 // device-side utils::unbroadcast: out[orig] (+)= sum over broadcast dims of grad[gshape]

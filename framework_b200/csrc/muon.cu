@@ -28,7 +28,10 @@ struct List {
     const float *grad[kMaxList];
     long long n[kMaxList];
     float scale[kMaxList];
+    uint16_t *planes[kMaxList];
+    long long plane[kMaxList];
     int rows[kMaxList], cols[kMaxList];
+    FastDiv vectors[kMaxList];                 // of 8 columns, in a row of the planes
     unsigned first[kMaxList + 1];              // index of a matrix's first chunk
     int chunk[kMaxList];                       // elements of one
     int count;
@@ -46,10 +49,12 @@ __device__ __forceinline__ int find(const List &list, unsigned chunk) {
 __device__ __forceinline__ float update_of(float g, float m, float mu, bool nesterov) { return nesterov ? fmaf(mu, m, g) : m; }
 
 __global__ void __launch_bounds__(kThreads)
-muon_momentum_kernel(const __grid_constant__ List list, float mu, bool nesterov, double *__restrict__ partial) {
+muon_momentum_kernel(const __grid_constant__ List list, float mu, bool nesterov, double *__restrict__ partial, unsigned *counters, int words) {
     __shared__ double red[8];
     grid_dependency_trigger();
     grid_dependency_wait();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < words; i += kThreads) counters[i] = 0u;
     const int t = find(list, blockIdx.x);
     const long long base = static_cast<long long>(blockIdx.x - list.first[t]) * list.chunk[t], end = min(list.n[t], base + list.chunk[t]);
     float *const m = list.momentum[t];
@@ -127,29 +132,24 @@ muon_update_kernel(const __grid_constant__ List list, float decay) {
     for (long long i = base + threadIdx.x; i < end; i += kThreads) p[i] = fmaf(-scale, x[i], decay * p[i]);
 }
 
-// x in f16 planes, hi + lo * 2^-12, 8 columns a thread; the matrices of a list are of one shape.  Bound by memory: 8 bytes read (4
-// without a momentum), 4 written.
-struct PlanesOut {
-    uint16_t *dst;
-    long long pitch, matrix, plane;
-    float scale;                               // 2^exponent
-    FastDiv vectors;                           // of a row
-    int first;                                 // index of the list's first matrix
-};
+// x in f16 planes, hi + lo * 2^-12, 8 columns a thread.  Bound by memory: 8 bytes read (4 without a momentum), 4 written.  scale: 2^exponent.
+// A block takes the same chunk of a matrix as above, counted in vectors.
 __global__ void __launch_bounds__(kThreads)
-muon_planes_kernel(const __grid_constant__ List list, float mu, bool nesterov, float eps, const double *__restrict__ partial, PlanesOut out,
-                   int per_block) {
+muon_planes_kernel(const __grid_constant__ List list, float mu, bool nesterov, float eps, const double *__restrict__ partial, float scale) {
     __shared__ double red[8];
     grid_dependency_trigger();
     grid_dependency_wait();
-    const int t = blockIdx.y, rows = list.rows[t], cols = list.cols[t];
-    const float factor = inverse_norm(list, t, partial, eps, red) * out.scale;
+    const int t = find(list, blockIdx.x), rows = list.rows[t], cols = list.cols[t];
+    const float factor = inverse_norm(list, t, partial, eps, red) * scale;
     const float *const m = list.momentum[t], *const g = list.grad[t];
-    uint16_t *const dst = out.dst + (out.first + t) * out.matrix;
+    uint16_t *const dst = list.planes[t];
+    const FastDiv per_row = list.vectors[t];
+    const int vectors = static_cast<int>(per_row.d) * rows, blocks = static_cast<int>(list.first[t + 1] - list.first[t]);
+    const int per_block = ((vectors + blocks - 1) / blocks + kThreads - 1) / kThreads * kThreads;
+    const int v0 = static_cast<int>(min(static_cast<long long>(vectors), static_cast<long long>(blockIdx.x - list.first[t]) * per_block)), v1 = min(vectors, v0 + per_block);
     const bool vec = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 && cols % 4 == 0;
-    const int vectors = static_cast<int>(out.vectors.d) * rows, v0 = blockIdx.x * per_block, v1 = min(vectors, v0 + per_block);
     for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
-        const int row = fd_div(v, out.vectors), col = (v - row * static_cast<int>(out.vectors.d)) * 8;
+        const int row = fd_div(v, per_row), col = (v - row * static_cast<int>(per_row.d)) * 8;
         const long long at = static_cast<long long>(row) * cols + col;
         float x[8], y[8];
         if (vec && col + 8 <= cols) {
@@ -181,9 +181,9 @@ muon_planes_kernel(const __grid_constant__ List list, float mu, bool nesterov, f
             h[i / 2] = *reinterpret_cast<const unsigned *>(&top);
             l[i / 2] = *reinterpret_cast<const unsigned *>(&rest);
         }
-        uint16_t *const to = dst + row * out.pitch + col;
+        uint16_t *const to = dst + static_cast<long long>(v) * 8;
         *reinterpret_cast<uint4 *>(to) = hi;
-        *reinterpret_cast<uint4 *>(to + out.plane) = lo;
+        *reinterpret_cast<uint4 *>(to + list.plane[t]) = lo;
     }
 }
 
@@ -209,6 +209,9 @@ int for_lists(const MuonEntry *e, int64_t count, Launch launch) {
             list.grad[k] = e[at].grad;
             list.n[k] = e[at].n;
             list.scale[k] = e[at].scale;
+            list.planes[k] = e[at].planes;
+            list.plane[k] = e[at].plane;
+            list.vectors[k] = make_fastdiv(std::max<int64_t>(1, e[at].pitch / 8));
             list.rows[k] = static_cast<int>(e[at].rows);
             list.cols[k] = static_cast<int>(e[at].cols);
             list.chunk[k] = static_cast<int>(chunk_of(e[at].n));
@@ -234,31 +237,21 @@ size_t muon_partial_bytes(const MuonEntry *e, int64_t count) {
     return static_cast<size_t>(chunks) * sizeof(double);
 }
 
-int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, const MuonPlanes &planes,
-                      cudaStream_t stream) {
+int launch_muon_start(const MuonEntry *e, int64_t count, float mu, bool nesterov, float eps, double *partial, int exponent, unsigned *counters,
+                      int words, cudaStream_t stream) {
     int rc = for_lists(e, count, [&](const List &list, unsigned chunks, int64_t before) -> int {
-        const cudaError_t r = launch_dependent(muon_momentum_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, partial + before);
+        const cudaError_t r = launch_dependent(muon_momentum_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, partial + before,
+                                               counters, words);
         if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_momentum_kernel launch failed: %s", cudaGetErrorString(r));
         MNI_LAUNCH_CHECK("muon_momentum_kernel");
         return MNI_B200_OK;
     });
     if (rc) return rc;
-    int first = 0;
     return for_lists(e, count, [&](const List &list, unsigned chunks, int64_t before) -> int {
         const double *const sums = partial + before;
-        cudaError_t r;
-        if (planes.dst) {
-            const int64_t row = planes.pitch / 8, vectors = row * list.rows[0];
-            // at least four vectors a thread of a large matrix, and blocks for some rounds where matrices are few
-            const int64_t blocks = std::min<int64_t>((vectors + kThreads - 1) / kThreads, std::max<int64_t>(1, 16ll * device_sm_count() / list.count));
-            const PlanesOut out{planes.dst, planes.pitch, planes.matrix, planes.plane, ldexpf(1.f, planes.exponent), make_fastdiv(row), first};
-            const int per = static_cast<int>(((vectors + blocks - 1) / blocks + kThreads - 1) / kThreads * kThreads);
-            r = launch_dependent(muon_planes_kernel, dim3(static_cast<unsigned>((vectors + per - 1) / per), static_cast<unsigned>(list.count)), dim3(kThreads), 0,
-                                 stream, list, mu, nesterov, eps, sums, out, per);
-        } else {
-            r = launch_dependent(muon_normalise_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, eps, sums);
-        }
-        first += list.count;
+        const cudaError_t r = list.planes[0]
+                                  ? launch_dependent(muon_planes_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, eps, sums, ldexpf(1.f, exponent))
+                                  : launch_dependent(muon_normalise_kernel, dim3(chunks), dim3(kThreads), 0, stream, list, mu, nesterov, eps, sums);
         if (r != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "muon_planes_kernel launch failed: %s", cudaGetErrorString(r));
         MNI_LAUNCH_CHECK("muon_planes_kernel");
         return MNI_B200_OK;
