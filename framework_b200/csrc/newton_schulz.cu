@@ -35,7 +35,7 @@ constexpr int kPieceBlocks = 2;                    // k-blocks whose large terms
 constexpr int kThreads = 32 * (4 + kEpiWarps);
 constexpr int kIssueRegs = 56, kEpiRegs = 224;     // of 168 a thread at launch
 static_assert(kIssueRegs + 2 * kEpiRegs <= 3 * 168, "more registers than the launch has");
-constexpr int kBars = 3 * kStagesMax + 4 + 2 * kRing;
+constexpr int kBars = 3 * kStagesMax + 4 + 2 * kRing + 1;
 constexpr int kFixedSmem = 1024 + kEpiWarps * kPatchBytes + kBars * 8 + 64;
 
 struct Group {
@@ -153,7 +153,8 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
     uint8_t *const patches = smem + static_cast<size_t>(p.stages) * STAGE;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(patches + kEpiWarps * kPatchBytes);
     const uint32_t bar_full = smem_u32(bars), bar_ready = bar_full + 8u * kStagesMax, bar_empty = bar_ready + 8u * kStagesMax,
-                   acc_full = bar_empty + 8u * kStagesMax, acc_empty = acc_full + 16u, unit_full = acc_empty + 16u, unit_empty = unit_full + 8u * kRing;
+                   acc_full = bar_empty + 8u * kStagesMax, acc_empty = acc_full + 16u, unit_full = acc_empty + 16u, unit_empty = unit_full + 8u * kRing,
+                   issued = unit_empty + 8u * kRing;
     volatile int *const ring = reinterpret_cast<int *>(bars + kBars);
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars) + kRing;
     volatile uint32_t *const abort_flag = tmem_slot + 1;
@@ -178,6 +179,7 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
             mbar_init(unit_full + 8u * i, 1);
             mbar_init(unit_empty + 8u * i, CG * (2 + kEpiWarps) + 1 + (CG == 2 ? 2 : 0));
         }
+        mbar_init(issued, 1);
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -317,12 +319,8 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                 }
             }
             if (!last) {                           // this warp's part is written: every lane's stores, before the count
-                asm volatile("fence.proxy.async;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    __threadfence();
-                    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + 3 * (g.first_matrix + t.matrix) + t.product) : "memory");
-                }
+                if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + 3 * (g.first_matrix + t.matrix) + t.product) : "memory");
             }
         }
     } else {
@@ -386,6 +384,7 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
                     }
                 }
+                if (!loads_a && rank == kDrawer && lane == 0) mbar_arrive(issued);
             }
             if (!ok) {                             // giving up: copies already issued land before the CTA exits
                 const int pending = min(armed, p.stages);
@@ -469,8 +468,14 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
             }
         } else if (warp == 2 ? CG == 2 : CG == 1) {
             // ------------------------------------------------------------ draws the units
+            // One at a time, when the copies of the one before are on their way: a CTA that held two tiles of a matrix's product while others
+            // had none made the chain of a single matrix half as long again (one of 256 x 256: 204 us).
             bool ok = true;
             for (int n = 0; ok; ++n) {
+                if (n > 0) {
+                    ok = mbar_wait_warp(issued, (n - 1) & 1, abort_flag, p.err, 0xa00u, unused, false, p.wait_cycles);
+                    if (!ok) break;
+                }
                 const int slot = n % kRing;
                 ok = wait_cluster(unit_empty + 8u * slot, ((n / kRing) & 1) ^ 1u, abort_flag, p.err, 0x900u | slot, p.wait_cycles);
                 ok = __all_sync(0xffffffffu, ok);
