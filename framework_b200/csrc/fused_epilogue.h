@@ -5,14 +5,12 @@
 //                 128 logits instead of 512 written and read again
 //   grad_chunk    z -> exp(z - lse) - [class = target], in planes for the two products that follow: 4 bytes instead of 4 + 4 + 4 + 4
 //                 through f32 logits, f32 gradients and a pass that splits them
-//   power_chunk   alpha * product + beta * identity -> planes, below the diagonal too where only tiles above it are computed; and
-//                 the same once more with other factors
 //
 // The kernel calls them chunk after chunk in a loop that is not unrolled, and moves the registers down in between: unrolled over 128
 // columns their code (40 KB, executed once a tile) came from beyond the instruction caches, and a tile's epilogue took 12 us.
 //
-// Planes are written row by row, 32 bytes a store of one thread: whole sectors.  Scales are fixed, not looked for: a gradient of
-// logits is at most one, what a polynomial makes is bounded on the host.
+// Planes are written row by row, 32 bytes a store of one thread: whole sectors.  The scale is fixed, not looked for: a gradient of
+// logits is at most one.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -25,9 +23,7 @@ namespace {
 struct FusedTile {
     int row, rows;                 // this thread's row, of so many
     int col, cols;                 // its first column, of so many
-    int batch;
     int stretch;                   // index of its columns' stretch
-    bool off_diagonal;
     int lane;
     float *patch;                  // 4 KB of shared memory of the warp's own
 };
@@ -176,67 +172,6 @@ __device__ __forceinline__ void grad_chunk(const FusedArgs &f, const FusedTile &
     store_planes16(dst + 16, hi + 8);
     store_planes16(dst + f.dst_plane, lo);
     store_planes16(dst + f.dst_plane + 16, lo + 8);
-}
-
-// Planes of alpha * product + beta on the diagonal, to one or two places.
-struct PowerOutputs {
-    long long dst_pitch, dst_matrix, dst_plane;
-    struct {
-        uint16_t *dst;
-        float alpha, beta;
-    } out[2];
-    int outputs;
-};
-__device__ __forceinline__ void power_chunk(const PowerOutputs &f, const FusedTile &at, const uint32_t (&v)[32], int c) {
-    const int col = at.col + 32 * c;
-    if (col >= at.cols) return;                    // the same for the whole warp
-    const int diagonal = at.row - col;
-    uint32_t *const patch = reinterpret_cast<uint32_t *>(at.patch);
-#pragma unroll 1
-    for (int i = 0; i < f.outputs; ++i) {
-        const float alpha = f.out[i].alpha, beta = f.out[i].beta;
-        uint16_t *const to = f.out[i].dst + at.batch * f.dst_matrix;
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2)
-            split_pair(fmaf(alpha, __uint_as_float(v[e]), diagonal == e ? beta : 0.f), fmaf(alpha, __uint_as_float(v[e + 1]), diagonal == e + 1 ? beta : 0.f),
-                       hi[e / 2], lo[e / 2]);
-        if (at.row < at.rows) {
-            uint16_t *const dst = to + at.row * f.dst_pitch + col;
-            store_planes16(dst, hi);
-            store_planes16(dst + f.dst_plane, lo);
-            if (col + 16 < at.cols) {              // (what lies between the last column and the pitch is never read as data)
-                store_planes16(dst + 16, hi + 8);
-                store_planes16(dst + f.dst_plane + 16, lo + 8);
-            }
-        }
-        if (at.off_diagonal) {
-            // 32 rows become 32 columns: (hi, lo) of an element in a word, turned in the warp's patch, no two lanes in one bank.
-            __syncwarp();
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                patch[at.lane * 32 + (e ^ at.lane)] = __byte_perm(hi[e / 2], lo[e / 2], 0x5410);
-                patch[at.lane * 32 + ((e + 1) ^ at.lane)] = __byte_perm(hi[e / 2], lo[e / 2], 0x7632);
-            }
-            __syncwarp();
-            const int row = at.row - at.lane;      // the first of the warp's rows; all of the result's pitch below
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                const uint32_t a = patch[e * 32 + (at.lane ^ e)], b = patch[(e + 1) * 32 + (at.lane ^ (e + 1))];
-                hi[e / 2] = __byte_perm(a, b, 0x5410);
-                lo[e / 2] = __byte_perm(a, b, 0x7632);
-            }
-            if (col + at.lane < at.cols && row < at.rows) {
-                uint16_t *const dst = to + static_cast<long long>(col + at.lane) * f.dst_pitch + row;
-                store_planes16(dst, hi);
-                store_planes16(dst + f.dst_plane, lo);
-                if (row + 16 < at.rows) {
-                    store_planes16(dst + 16, hi + 8);
-                    store_planes16(dst + f.dst_plane + 16, lo + 8);
-                }
-            }
-        }
-    }
 }
 
 }  // namespace

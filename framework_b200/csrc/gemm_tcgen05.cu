@@ -661,7 +661,7 @@ gemm_tc_kernel(const __grid_constant__ KernelArgs<MODE, TAIL> g) {
                 if (!last_piece) continue;
             }
             if constexpr (is_fused(TAIL)) {
-                const FusedTile at{row0 + lane, q.M, t.tn * BN + chunk_lo * 32, q.N, t.bt, t.tn * 2 + (ew >> 2), t.tm != t.tn, lane,
+                const FusedTile at{row0 + lane, q.M, t.tn * BN + chunk_lo * 32, q.N, t.tn * 2 + (ew >> 2), lane,
                                    reinterpret_cast<float *>(my_stage)};
                 auto chunks = [&](auto body) {     // one chunk's code for all of them
 #pragma unroll 1
@@ -1772,7 +1772,8 @@ int make_half_map(CUtensorMap *map, const HalfOperand &op, int *mode, int box_ro
         box[1] = 64; box[2] = static_cast<cuuint32_t>(box_rows / 64);
         *mode = kMnSingleBox;
     }
-    const CUresult r = encode(map, op.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    if (box_rows == 32) box[0] = 32;                    // what an epilogue warp writes
+    const CUresult r = encode(map, op.ptr, dims, strides, box, box_rows == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
     if (r != CUDA_SUCCESS) return fail(MNI_B200_ERR_CUDA, "cuTensorMapEncodeTiled(halves) failed (%d)", static_cast<int>(r));
     return MNI_B200_OK;
 }

@@ -138,8 +138,8 @@ struct HalfOperand {
 };
 // lo = (x - hi) * 2^kHalfLoShift: the whole range of f16 serves the part below hi's last bit
 constexpr int kHalfLoShift = 12;
-// Tensor map of an operand in planes: boxes of 64 contraction elements by box_rows (64 or 128), swizzled; coordinates (k, row, batch,
-// plane, 0), or for an MN-major one (0, k, row / 64, batch, plane).
+// Tensor map of an operand in planes: boxes of 64 contraction elements by box_rows (64 or 128), 128-byte swizzle; coordinates (k, row, batch,
+// plane, 0), or for an MN-major one (0, k, row / 64, batch, plane).  box_rows 32: 32 by 32 elements, 64-byte swizzle, for stores.
 int half_operand_map(CUtensorMap *map, const HalfOperand &op, int box_rows);
 // f16 planes: exponents lie within this either way.
 constexpr int kHalfMaxExp = 60;
@@ -404,7 +404,7 @@ struct NewtonProblem {
 struct NewtonStep {
     float a, r, r_diagonal, q, q_diagonal, x;
 };
-constexpr int kNewtonGroups = 12, kNewtonMatrices = 512, kNewtonSteps = 100;      // of a launch (25 KB of kernel parameters)
+constexpr int kNewtonGroups = 8, kNewtonMatrices = 512, kNewtonSteps = 100;      // of a launch (25 KB of kernel parameters)
 // out[i] = x of matrix i, or (update) decay * out[i] - scale[i] * x.  counters: 1 + 3 * matrices words, zero.
 int launch_newton_schulz(const NewtonProblem *problems, int count, const NewtonStep *steps, int step_count, float *const *out, const float *scale, bool update,
                          float decay, unsigned *counters, uint32_t *err_word, int sm_count, cudaStream_t stream);

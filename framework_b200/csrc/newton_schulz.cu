@@ -12,8 +12,12 @@
 //   warp 0, 1   TMA producers of A and of B (both wait for the unit's matrix, then order the other CTAs' stores before their copies)
 //   warp 2      issues the MMAs (of a pair: the leader's; the peer's draws the units)
 //   warp 3      pair: relays "landed" to the leader; lone CTA: draws the units
-//   warp 4-11   epilogue: planes of the result, above and below the diagonal where it is symmetric (only tiles on and above it are
-//               computed), or f32: the orthogonal matrix, or the parameter that it updates
+//   warp 4-11   epilogue: planes of the result, by TMA from the warp's patch, or f32: the orthogonal matrix, or the parameter that it
+//               updates.  Plain stores of a thread's own row (32 rows a store) took 70 clocks each, 11000 for a 256 x 256 tile, in which
+//               nobody drained the next tile's accumulators.
+//
+// Of a symmetric result only the tiles on and above the diagonal are computed, and only they are written: a block of 64 contraction elements
+// that lies below is loaded from above and given to the tensor core as what it is, MN-major.
 //
 // Tiles: 256 x 256 of a pair (24.4 clocks an element of the contraction: the pipe's 24), 128 x 128 of a lone CTA (24: its shared memory
 // feeds half of the pipe) or 128 x 64 (15).  The smaller ones have less to do in the chain of a single matrix, the large ones do twice as
@@ -39,9 +43,9 @@ constexpr int kBars = 3 * kStagesMax + 4 + 2 * kRing + 1;
 constexpr int kFixedSmem = 1024 + kEpiWarps * kPatchBytes + kBars * 8 + 64;
 
 struct Group {
-    CUtensorMap a1[2], b1[2], a2, b2, q3, x3[2];   // [2]: by the step's parity
-    uint16_t *x[2], *a, *r, *q;
-    long long x_pitch, x_matrix, x_plane, s_pitch, s_matrix, s_plane;
+    CUtensorMap a1[2], b1[2], x3[2];               // x, by the step's parity
+    CUtensorMap a2[2], b2[2], q3[2];               // A, R and Q, contraction along rows and along columns
+    CUtensorMap to_x[2], to_a, to_r, to_q;         // what the epilogue writes
     int rows, cols, side, count, tall;
     int first_matrix;
     int tiles1, tn1, tm3, tn3;                     // tiles of a symmetric product (on and above the diagonal), its columns of tiles; of x
@@ -67,7 +71,6 @@ struct Args {
 
 struct Unit {
     int step, product, matrix, tm, tn;             // matrix: within the group
-    bool off_diagonal;
     const Group *g;
 };
 template <int RATIO>
@@ -91,19 +94,35 @@ __device__ __forceinline__ Unit decode(const Args &p, int u) {
             ++t.tm;
         }
         t.tn = RATIO * t.tm + r;
-        t.off_diagonal = t.tn >= RATIO * (t.tm + 1);
     } else {
         const int tiles = t.g->tm3 * t.g->tn3;
         t.matrix = r / tiles;
         r -= t.matrix * tiles;
         t.tn = r / t.g->tm3;
         t.tm = r - t.tn * t.g->tm3;
-        t.off_diagonal = false;
     }
     return t;
 }
 __device__ __forceinline__ int contraction(const Unit &t) {
     return t.product == 0 ? (t.g->tall ? t.g->rows : t.g->cols) : t.g->side;
+}
+
+// How an operand's block of 64 contraction elements lies in memory.  Of a symmetric matrix the blocks of `TM` rows below the diagonal are
+// never written: they are read as what lies above it, turned.
+struct Major {
+    bool symmetric, mn;
+    int block;                                     // of TM rows
+    template <int TM>
+    __device__ __forceinline__ bool mn_at(int it) const { return symmetric ? it / (TM / BK) < block : mn; }
+};
+template <int RATIO>
+__device__ __forceinline__ Major major_of(const Unit &t, bool of_a) {
+    const bool tall = t.g->tall != 0;
+    Major m;
+    m.symmetric = t.product == 1 || (t.product == 2 && tall != of_a);
+    m.mn = t.product == 0 ? tall : !of_a;          // (of x: behind Q it is read along its rows, before Q along its columns)
+    m.block = of_a ? t.tm : t.tn / RATIO;
+    return m;
 }
 
 // Waits with the reach of a cluster, for what another CTA of it has stored before it arrived.
@@ -248,6 +267,29 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                 }
             }
         };
+        // alpha * (the first chunk of run) + beta on the diagonal, in planes, to where `map` lies: a half of the patch each
+        auto put = [&](const CUtensorMap *map, float alpha, float beta, int diagonal, int col, int row, int matrix) {
+            uint32_t x[2][16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+                split_pair(fmaf(alpha, __uint_as_float(run[0][e]), diagonal == e ? beta : 0.f),
+                           fmaf(alpha, __uint_as_float(run[0][e + 1]), diagonal == e + 1 ? beta : 0.f), x[0][e / 2], x[1][e / 2]);
+#pragma unroll
+            for (int plane = 0; plane < 2; ++plane) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // what this half held has been read
+                __syncwarp();
+                uint8_t *const to = reinterpret_cast<uint8_t *>(patch) + plane * (kPatchBytes / 2) + lane * 64;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<uint4 *>(to + ((k ^ ((lane >> 1) & 3)) * 16)) = make_uint4(x[plane][4 * k], x[plane][4 * k + 1], x[plane][4 * k + 2], x[plane][4 * k + 3]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_planes(map, smem_u32(patch) + plane * (kPatchBytes / 2), col, row, matrix, plane);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+            }
+        };
         for (int n = 0; ok; ++n) {
             const int u = next_unit(n);
             if (u < 0) break;
@@ -269,46 +311,45 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
             const bool of_x = t.product == 2, last = of_x && t.step + 1 == p.steps;
             const int rows = of_x ? g.rows : g.side, cols = of_x ? g.cols : g.side;
             const int row0 = t.tm * TM + static_cast<int>(rank) * BM + quarter * 32;
-            const FusedTile at{row0 + lane, rows, t.tn * BN + half * (BN / 2), cols, t.matrix, 0, t.off_diagonal, lane, patch};
+            const int col0 = t.tn * BN + half * (BN / 2);
             const Step &s = p.step[t.step];
-            PowerOutputs f;
-            f.dst_pitch = of_x ? g.x_pitch : g.s_pitch;
-            f.dst_matrix = of_x ? g.x_matrix : g.s_matrix;
-            f.dst_plane = of_x ? g.x_plane : g.s_plane;
-            f.outputs = t.product == 0 ? 2 : 1;
-            f.out[0].dst = t.product == 0 ? g.a : t.product == 1 ? g.q : g.x[(t.step + 1) & 1];
-            f.out[0].alpha = t.product == 0 ? s.a : t.product == 1 ? s.q : s.x;
-            f.out[0].beta = t.product == 1 ? s.q_diagonal : 0.f;
-            f.out[1].dst = g.r;
-            f.out[1].alpha = s.r;
-            f.out[1].beta = s.r_diagonal;
+            const int m = g.first_matrix + t.matrix;
             if (row0 < rows) {
 #pragma unroll 1
                 for (int c = 0; c < CHUNKS; ++c) {
+                    const int col = col0 + 32 * c;
+                    if (col >= cols) break;
                     if (!last) {
-                        power_chunk(f, at, run[0], c);
-                    } else if (at.col + 32 * c < cols) {
+                        const int diagonal = row0 + lane - col;
+                        if (t.product == 0) {
+                            put(&g.to_a, s.a, 0.f, diagonal, col, row0, t.matrix);
+                            put(&g.to_r, s.r, s.r_diagonal, diagonal, col, row0, t.matrix);
+                        } else if (t.product == 1) {
+                            put(&g.to_q, s.q, s.q_diagonal, diagonal, col, row0, t.matrix);
+                        } else {
+                            put(&g.to_x[(t.step + 1) & 1], s.x, 0.f, diagonal, col, row0, t.matrix);
+                        }
+                    } else {
                         // the result in f32: turned in the patch, so that a store covers 32 neighbouring columns whatever the alignment
+                        float *const out = p.out[m] + static_cast<long long>(row0) * cols + col + lane;
+                        const float scale = p.scale[m];
+                        const int live = col + lane < cols ? min(32, rows - row0) : 0;
                         __syncwarp();
 #pragma unroll
                         for (int e = 0; e < 32; ++e) patch[lane * 32 + (e ^ lane)] = __uint_as_float(run[0][e]) * s.x;
                         __syncwarp();
-                        const int col = at.col + 32 * c + lane, m = g.first_matrix + t.matrix;
-                        float *const out = p.out[m] + static_cast<long long>(row0) * cols + col;
-                        const float scale = p.scale[m];
-                        if (col < cols) {
-#pragma unroll 1
-                            for (int r0 = 0; r0 < 32; r0 += 8) {
-                                float y[8];
-                                if (p.update) {
+                        constexpr int AT_ONCE = CHUNKS > 2 ? 16 : 32;              // loads in flight: as registers allow
 #pragma unroll
-                                    for (int r = 0; r < 8; ++r) y[r] = row0 + r0 + r < rows ? out[static_cast<long long>(r0 + r) * cols] : 0.f;
-                                }
+                        for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+                            float y[AT_ONCE];
+                            if (p.update) {
 #pragma unroll
-                                for (int r = 0; r < 8; ++r) {
-                                    const float v = patch[(r0 + r) * 32 + (lane ^ (r0 + r))];
-                                    if (row0 + r0 + r < rows) out[static_cast<long long>(r0 + r) * cols] = p.update ? fmaf(-scale, v, p.decay * y[r]) : v;
-                                }
+                                for (int r = 0; r < AT_ONCE; ++r) y[r] = r0 + r < live ? out[static_cast<long long>(r0 + r) * cols] : 0.f;
+                            }
+#pragma unroll
+                            for (int r = 0; r < AT_ONCE; ++r) {
+                                const float v = patch[(r0 + r) * 32 + (lane ^ (r0 + r))];
+                                if (r0 + r < live) out[static_cast<long long>(r0 + r) * cols] = p.update ? fmaf(-scale, v, p.decay * y[r]) : v;
                             }
                         }
                     }
@@ -318,9 +359,12 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                         for (int e = 0; e < 32; ++e) run[d - 1][e] = run[d][e];
                 }
             }
-            if (!last) {                           // this warp's part is written: every lane's stores, before the count
+            if (!last) {                           // this warp's part is written, before the count
+                if (lane == 0) {
+                    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+                    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + 3 * m + t.product) : "memory");
+                }
                 __syncwarp();
-                if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.done + 3 * (g.first_matrix + t.matrix) + t.product) : "memory");
             }
         }
     } else {
@@ -362,12 +406,13 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                     asm volatile("fence.proxy.async;" ::: "memory");       // their stores before the copies of whichever lane issues them
                 }
                 const int blocks = (contraction(t) + BK - 1) / BK, parity = t.step & 1;
-                // MN-major operands: x x^T of x^T x's, and x behind Q
-                const bool mn = loads_a ? t.product == 0 && g.tall : (t.product == 0 && g.tall) || (t.product == 2 && !g.tall);
-                const CUtensorMap *const map = loads_a ? (t.product == 0 ? &g.a1[parity] : t.product == 1 ? &g.a2 : g.tall ? &g.x3[parity] : &g.q3)
-                                                       : (t.product == 0 ? &g.b1[parity] : t.product == 1 ? &g.b2 : g.tall ? &g.q3 : &g.x3[parity]);
+                const Major major = major_of<RATIO>(t, loads_a);
+                const CUtensorMap *const along = loads_a ? (t.product == 0 ? &g.a1[parity] : t.product == 1 ? &g.a2[0] : g.tall ? &g.x3[parity] : &g.q3[0])
+                                                         : (t.product == 0 ? &g.b1[parity] : t.product == 1 ? &g.b2[0] : g.tall ? &g.q3[0] : &g.x3[parity]);
                 const int row = loads_a ? t.tm * TM + static_cast<int>(rank) * BM : t.tn * BN + static_cast<int>(rank) * BNL;
                 for (int it = 0; ok && it < blocks; ++it) {
+                    const bool mn = major.mn_at<TM>(it);
+                    const CUtensorMap *const map = along + (major.symmetric && mn ? 1 : 0);
                     for (int plane = 0; plane < 2; ++plane) {
                         ok = mbar_wait_warp(bar_empty + 8u * stage, phase ^ 1u, abort_flag, p.err, 0x100u | stage, unused, false, p.wait_cycles);
                         if (!ok) break;
@@ -406,13 +451,14 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                 const int u = next_unit(n);
                 if (u < 0) break;
                 const Unit t = decode<RATIO>(p, u);
-                const bool a_mn = t.product == 0 && t.g->tall, b_mn = a_mn || (t.product == 2 && !t.g->tall);
-                const uint32_t lbo = static_cast<uint32_t>((BK * 128) >> 4) << 16;                 // MN-major: chunks of 64 rows
-                const uint32_t a0 = sa | (a_mn ? lbo : 0u), b0 = sb | (b_mn ? lbo : 0u), a_ks = a_mn ? 128u : 2u, b_ks = b_mn ? 128u : 2u;
-                const uint32_t idesc = (1u << 4) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(BN >> 3) << 17) |
-                                       (static_cast<uint32_t>(TM >> 4) << 24);
+                const Major a_major = major_of<RATIO>(t, true), b_major = major_of<RATIO>(t, false);
                 const int blocks = (contraction(t) + BK - 1) / BK;
                 for (int it = 0; it < blocks; ++it) {
+                    const bool a_mn = a_major.mn_at<TM>(it), b_mn = b_major.mn_at<TM>(it);
+                    const uint32_t lbo = static_cast<uint32_t>((BK * 128) >> 4) << 16;             // MN-major: chunks of 64 rows
+                    const uint32_t a0 = sa | (a_mn ? lbo : 0u), b0 = sb | (b_mn ? lbo : 0u), a_ks = a_mn ? 128u : 2u, b_ks = b_mn ? 128u : 2u;
+                    const uint32_t idesc = (1u << 4) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(BN >> 3) << 17) |
+                                           (static_cast<uint32_t>(TM >> 4) << 24);
                     const int in_piece = it % kPieceBlocks;
                     const bool begins = in_piece == 0, last = it + 1 == blocks, ends = last || in_piece + 1 == kPieceBlocks, large_first = ends && !last;
                     ok = mbar_wait_warp(ready + 8u * stage, phase, abort_flag, p.err, 0x300u | stage, unused, false, p.wait_cycles);
@@ -623,9 +669,6 @@ int launch_newton_schulz(const NewtonProblem *problems, int count, const NewtonS
         g.tall = n.tall() ? 1 : 0;
         g.first_matrix = matrices;
         matrices += g.count;
-        g.x[0] = n.x[0]; g.x[1] = n.x[1]; g.a = n.a; g.r = n.r; g.q = n.q;
-        g.x_pitch = n.x_pitch; g.x_matrix = n.rows * n.x_pitch; g.x_plane = g.x_matrix * n.count;
-        g.s_pitch = n.s_pitch; g.s_matrix = n.side() * n.s_pitch; g.s_plane = g.s_matrix * n.count;
         g.tiles1 = static_cast<int>(t1);
         g.tn1 = static_cast<int>((n.side() + t.bn - 1) / t.bn);
         g.tm3 = static_cast<int>(tm3);
@@ -643,21 +686,29 @@ int launch_newton_schulz(const NewtonProblem *problems, int count, const NewtonS
             o.rows = k_major ? rows : cols;
             o.kdim = k_major ? cols : rows;
             o.pitch = of_x ? n.x_pitch : n.s_pitch;
-            o.matrix = of_x ? g.x_matrix : g.s_matrix;
-            o.plane = of_x ? g.x_plane : g.s_plane;
+            o.matrix = rows * o.pitch;
+            o.plane = o.matrix * n.count;
             o.batch = n.count;
             o.planes = 2;
             return o;
         };
         const int b_rows = t.bn / t.cg;
-        int rc = half_operand_map(&g.a2, operand(n.a, false, true), 128);
-        if (rc == MNI_B200_OK) rc = half_operand_map(&g.b2, operand(n.r, false, true), b_rows);
-        if (rc == MNI_B200_OK) rc = half_operand_map(&g.q3, operand(n.q, false, true), n.tall() ? b_rows : 128);
-        for (int k = 0; k < 2 && rc == MNI_B200_OK; ++k) {
-            rc = half_operand_map(&g.a1[k], operand(n.x[k], true, !n.tall()), 128);
-            if (rc == MNI_B200_OK) rc = half_operand_map(&g.b1[k], operand(n.x[k], true, !n.tall()), b_rows);
-            if (rc == MNI_B200_OK) rc = half_operand_map(&g.x3[k], operand(n.x[k], true, n.tall()), n.tall() ? 128 : b_rows);
+        int rc = MNI_B200_OK;
+        auto map = [&](CUtensorMap *to, const uint16_t *ptr, bool of_x, bool k_major, int box_rows) {
+            if (rc == MNI_B200_OK) rc = half_operand_map(to, operand(ptr, of_x, k_major), box_rows);
+        };
+        for (int k = 0; k < 2; ++k) {
+            map(&g.a1[k], n.x[k], true, !n.tall(), 128);
+            map(&g.b1[k], n.x[k], true, !n.tall(), b_rows);
+            map(&g.x3[k], n.x[k], true, n.tall(), n.tall() ? 128 : b_rows);
+            map(&g.a2[k], n.a, false, k == 0, 128);
+            map(&g.b2[k], n.r, false, k == 0, b_rows);
+            map(&g.q3[k], n.q, false, k == 0, n.tall() ? b_rows : 128);
+            map(&g.to_x[k], n.x[k], true, true, 32);
         }
+        map(&g.to_a, n.a, false, true, 32);
+        map(&g.to_r, n.r, false, true, 32);
+        map(&g.to_q, n.q, false, true, 32);
         if (rc) return rc;
     }
     if (matrices > kNewtonMatrices) return fail(MNI_B200_ERR_ARG, "internal: too many matrices for a launch");

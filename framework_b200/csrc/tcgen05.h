@@ -110,6 +110,11 @@ __device__ __forceinline__ void tma_store_5d(const CUtensorMap *map, uint32_t sr
                  ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(0), "r"(0)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store_planes(const CUtensorMap *map, uint32_t src, int col, int row, int matrix, int plane) {
+    asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(col), "r"(row), "r"(matrix), "r"(plane), "r"(0)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_reduce_add_5d(const CUtensorMap *map, uint32_t src, int c0, int c1, int c2) {
     asm volatile(
         "cp.reduce.async.bulk.tensor.5d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
