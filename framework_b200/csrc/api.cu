@@ -1381,6 +1381,11 @@ int loss_fwd_body(Call &c, const LossCall &l, float *loss, float *lse) {
     const size_t sums_at = c.arena.reserve(loss_sums_bytes(l.M));
     float2 *const pairs = reinterpret_cast<float2 *>(c.dry() ? dry_pointer() : c.at(pairs_at));
     float *const picked = c.dry() ? dry_pointer() : c.at(picked_at);
+    if (!planes && small_logits(l.M, l.K, l.N)) {
+        if (c.dry()) return MNI_B200_OK;
+        const int r = launch_small_logits(rows_in(l), l.w->ptr, l.w->stride[0], l.w->stride[1], l.bias, l.N, l.targets, pairs, picked, c.stream);
+        return r ? r : launch_loss_finish(pairs, 1, l.M, l.N, l.targets, picked, l.reduction, loss, lse, reinterpret_cast<double2 *>(c.at(sums_at)), c.stream);
+    }
     mni_b200_view x, packed[2];
     int rc = rows_of_x(c, l, x);
     if (rc) return rc;
@@ -1428,7 +1433,8 @@ int loss_bwd_small(Call &c, const LossCall &l, const float *lse, const float *gr
     x.shape[0] = l.M; x.shape[1] = l.K;
     x.stride[0] = l.K; x.stride[1] = 1;
     int rc = MNI_B200_OK;
-    if (!c.dry()) {
+    const bool together = small_logits(l.M, l.K, l.N);
+    if (!c.dry() && !together) {
         rc = launch_row_weights(rows_in(l), l.targets, l.reduction, grad, reinterpret_cast<int *>(c.at(count)), c.at(weights), c.at(copy), false,
                                 nullptr, c.st->sm_count, c.stream);
         if (rc) return rc;
@@ -1441,8 +1447,14 @@ int loss_bwd_small(Call &c, const LossCall &l, const float *lse, const float *gr
     z.stride[0] = l.N; z.stride[1] = 1;
     const uint32_t flags = c.flags;
     c.flags = 0;
-    rc = fwd_body(c, &x, l.w, const_cast<float *>(z.ptr), l.bias);
-    if (rc == MNI_B200_OK && !c.dry()) rc = launch_logit_grad(const_cast<float *>(z.ptr), l.M, l.N, l.targets, lse, c.at(weights), c.stream);
+    if (together) {
+        if (!c.dry())
+            rc = launch_small_grads(rows_in(l), l.w->ptr, l.w->stride[0], l.w->stride[1], l.bias, l.N, l.targets, l.reduction, lse, grad,
+                                    const_cast<float *>(z.ptr), c.at(copy), c.stream);
+    } else {
+        rc = fwd_body(c, &x, l.w, const_cast<float *>(z.ptr), l.bias);
+    }
+    if (rc == MNI_B200_OK && !c.dry() && !together) rc = launch_logit_grad(const_cast<float *>(z.ptr), l.M, l.N, l.targets, lse, c.at(weights), c.stream);
     c.flags = flags & (MNI_B200_ACCUMULATE_DA | MNI_B200_ACCUMULATE_DB | MNI_B200_ACCUMULATE_DBIAS);
     if (rc == MNI_B200_OK && !turned) rc = bwd_body(c, &x, l.w, &z, dx, dw, dbias);
     if (rc == MNI_B200_OK && turned) {

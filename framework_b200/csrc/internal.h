@@ -360,6 +360,12 @@ struct RowsIn {
 constexpr int kLogitStretch = 2048;    // logits of a row that one block joins into a pair (maximum, sum of exponentials)
 // pairs[stretch][row]; at_target[row] is written where this call's classes include the target
 int launch_logit_stats(const float *z, int64_t rows, int64_t n, const Targets &targets, float2 *pairs, float *at_target, cudaStream_t stream);
+// The logits of few short rows and their pairs (one a row), or their weighted gradients d and the copy of x that dw is made of, in a launch.
+bool small_logits(int64_t rows, int64_t k, int64_t n);
+int launch_small_logits(const RowsIn &x, const float *w, int64_t w_k, int64_t w_n, const float *bias, int64_t n, const Targets &targets, float2 *pairs,
+                        float *at_target, cudaStream_t stream);
+int launch_small_grads(const RowsIn &x, const float *w, int64_t w_k, int64_t w_n, const float *bias, int64_t n, const Targets &targets, int reduction,
+                       const float *lse, const float *grad, float *d, float *copy, cudaStream_t stream);
 size_t loss_sums_bytes(int64_t rows);
 int launch_loss_finish(const float2 *pairs, int64_t parts, int64_t rows, int64_t classes, const Targets &targets, const float *at_target,
                        int reduction, float *loss, float *lse, double2 *sums, cudaStream_t stream);

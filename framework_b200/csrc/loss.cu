@@ -218,6 +218,81 @@ row_weights_kernel(const __grid_constant__ RowsIn x, Targets targets, int reduct
     }
 }
 
+// Logits of a row that a block computes itself, for few logits of short rows: a pair and the target's logit (GRAD false), or the weighted
+// gradient g * (exp(z - lse) - [j = t]) and the copy of x that dw is made of, zero in rows left out.  Each column is summed by `256 >> shift`
+// threads, whose sums are added in order.  Bound by latency: one launch where product, logits' pass and (GRAD) weights are two or three.
+template <bool GRAD>
+__global__ void __launch_bounds__(kThreads)
+small_logits_kernel(const __grid_constant__ RowsIn x, const float *__restrict__ w, long long w_k, long long w_n, const float *__restrict__ bias, int n,
+                    int shift, Targets targets, float2 *__restrict__ pairs, float *__restrict__ at_target, int reduction, const float *__restrict__ lse,
+                    const float *__restrict__ grad, float *__restrict__ d, float *__restrict__ copy) {
+    extern __shared__ float row_of[];
+    __shared__ float part[kThreads];
+    __shared__ int red[32];
+    float *const xs = row_of, *const zs = row_of + x.cols;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int row = blockIdx.x;
+    const long long t = target_at(targets, row);
+    const bool kept = !GRAD || t >= 0;
+    const float *const src = x.ptr + x.offset(row);
+    for (int c = threadIdx.x; c < x.cols; c += kThreads) {
+        const float v = kept ? src[c * x.col_stride] : 0.f;
+        xs[c] = v;
+        if (GRAD) copy[static_cast<long long>(row) * x.cols + c] = v;
+    }
+    float g = 0.f;
+    if (GRAD) {
+        g = reduction == 0 ? grad[row] : grad[0];
+        if (reduction == 2) g /= static_cast<float>(count_rows(targets, x.rows, red));
+    }
+    __syncthreads();
+    const int cols = 1 << shift, groups = kThreads >> shift, col = threadIdx.x & (cols - 1), group = threadIdx.x >> shift;
+    for (int j0 = 0; j0 < n; j0 += cols) {
+        const int j = j0 + col;
+        float z = 0.f;
+        if (j < n) {
+            const float *const at = w + j * w_n;
+#pragma unroll 8
+            for (int k = group; k < x.cols; k += groups) z = fmaf(xs[k], __ldg(at + k * w_k), z);
+        }
+        if (groups > 1) {                          // (the row is one round of columns then)
+            part[threadIdx.x] = z;
+            __syncthreads();
+            for (int i = 1; i < groups; ++i) z += part[(i << shift) + col];
+        }
+        if (group == 0 && j < n) zs[j] = bias ? z + __ldg(bias + j) : z;
+    }
+    __syncthreads();
+    if (GRAD) {
+        const float l = lse[row];
+        for (int c = threadIdx.x; c < n; c += kThreads) {
+            const float e = expf(zs[c] - l) - (c == t ? 1.f : 0.f);
+            d[static_cast<long long>(row) * n + c] = t < 0 ? 0.f : t < n ? e * g : NAN;
+        }
+        return;
+    }
+    float m = -INFINITY;
+    for (int c = threadIdx.x; c < n; c += kThreads) m = fmaxf(m, zs[c]);
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = part[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, part[i]);
+    const float to = isinf(m) ? 0.f : m;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < n; c += kThreads) s += expf(zs[c] - to);
+    s = warp_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < 8; ++i) s += part[i];
+    pairs[row] = make_float2(m, s);
+    if (t >= 0 && t < n) at_target[row] = zs[t];
+}
+
 // z -> g * (exp(z - lse) - [j = t]), in place.
 __global__ void __launch_bounds__(kThreads)
 logit_grad_kernel(float *__restrict__ z, int n, FastDiv stretches, Targets targets, const float *__restrict__ lse,
@@ -384,6 +459,41 @@ int launch_row_weights(const RowsIn &x, const Targets &targets, int reduction, c
                                            weights, copy, scaled ? 1 : 0, grad_exponent);
     if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "row_weights_kernel launch failed: %s", cudaGetErrorString(e));
     MNI_LAUNCH_CHECK("row_weights_kernel");
+    return MNI_B200_OK;
+}
+
+static int small_shift(int64_t n) {
+    int shift = 5;
+    while (shift < 8 && (1 << shift) < n) ++shift;
+    return shift;
+}
+// What small_logits_kernel takes: rows whose threads wait for weights four times at most (eight loads at a time).  us, product and passes / this: a
+// step of 32 rows, 64 features and 96 classes 28.5 / 21.9; from a graph its gradient 10.4 / 8.3 and the loss 7.8 / 7.8.  With eight waits (128
+// features, 128 classes) 9.7 / 10.9 for the loss and 12.4 / 11.1 for the gradient, with sixteen (1024 features, 16 classes) 8.9 / 16.2 and
+// 11.1 / 14.1.
+bool small_logits(int64_t rows, int64_t k, int64_t n) {
+    const int64_t cols = int64_t{1} << small_shift(n), groups = kThreads / cols;
+    return rows <= kCountRows && (n + cols - 1) / cols * ((k + 8 * groups - 1) / (8 * groups)) <= 4;
+}
+
+int launch_small_logits(const RowsIn &x, const float *w, int64_t w_k, int64_t w_n, const float *bias, int64_t n, const Targets &targets, float2 *pairs,
+                        float *at_target, cudaStream_t stream) {
+    const cudaError_t e = launch_dependent(small_logits_kernel<false>, dim3(static_cast<unsigned>(x.rows)), dim3(kThreads),
+                                           static_cast<size_t>(x.cols + n) * sizeof(float), stream, x, w, static_cast<long long>(w_k),
+                                           static_cast<long long>(w_n), bias, static_cast<int>(n), small_shift(n), targets, pairs, at_target, 0, nullptr,
+                                           nullptr, nullptr, nullptr);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "small_logits_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("small_logits_kernel");
+    return MNI_B200_OK;
+}
+int launch_small_grads(const RowsIn &x, const float *w, int64_t w_k, int64_t w_n, const float *bias, int64_t n, const Targets &targets, int reduction,
+                       const float *lse, const float *grad, float *d, float *copy, cudaStream_t stream) {
+    const cudaError_t e = launch_dependent(small_logits_kernel<true>, dim3(static_cast<unsigned>(x.rows)), dim3(kThreads),
+                                           static_cast<size_t>(x.cols + n) * sizeof(float), stream, x, w, static_cast<long long>(w_k),
+                                           static_cast<long long>(w_n), bias, static_cast<int>(n), small_shift(n), targets, nullptr, nullptr, reduction, lse,
+                                           grad, d, copy);
+    if (e != cudaSuccess) return fail(MNI_B200_ERR_CUDA, "small_logits_kernel launch failed: %s", cudaGetErrorString(e));
+    MNI_LAUNCH_CHECK("small_logits_kernel");
     return MNI_B200_OK;
 }
 
