@@ -94,8 +94,12 @@ muon_momentum_kernel(const __grid_constant__ List list, float mu, bool nesterov,
     }
 }
 
-// 1 / (norm + eps) of matrix t, from its chunks' sums: the same in every block that asks.
-__device__ float inverse_norm(const List &list, int t, const double *partial, float eps, double *red) {
+// 1 / (norm + eps) of matrix t, from its chunks' sums, as two factors near its root: of matrices whose norm or its inverse is beyond f32's normal
+// range neither they nor what has been multiplied by the first is.  The same in every block that asks.
+struct Inverse {
+    float first, second;
+};
+__device__ Inverse inverse_norm(const List &list, int t, const double *partial, float eps, double *red) {
     double sum = 0.0;
     for (unsigned i = list.first[t] + threadIdx.x; i < list.first[t + 1]; i += kThreads) sum += __ldcg(partial + i);
 #pragma unroll
@@ -104,7 +108,10 @@ __device__ float inverse_norm(const List &list, int t, const double *partial, fl
     __syncthreads();
     sum = red[0];
     for (int w = 1; w < 8; ++w) sum += red[w];
-    return static_cast<float>(1.0 / (sqrt(sum) + static_cast<double>(eps)));
+    const double inverse = 1.0 / (sqrt(sum) + static_cast<double>(eps));
+    if (!(inverse > 0.0) || isinf(inverse)) return Inverse{1.f, static_cast<float>(inverse)};
+    const double first = ldexp(1.0, ilogb(inverse) / 2);
+    return Inverse{static_cast<float>(first), static_cast<float>(inverse / first)};
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -113,11 +120,11 @@ muon_normalise_kernel(const __grid_constant__ List list, float mu, bool nesterov
     grid_dependency_trigger();
     grid_dependency_wait();
     const int t = find(list, blockIdx.x);
-    const float inverse = inverse_norm(list, t, partial, eps, red);
+    const Inverse inverse = inverse_norm(list, t, partial, eps, red);
     const long long base = static_cast<long long>(blockIdx.x - list.first[t]) * list.chunk[t], end = min(list.n[t], base + list.chunk[t]);
     const float *const m = list.momentum[t], *const g = list.grad[t];
     float *const x = list.x[t];
-    for (long long i = base + threadIdx.x; i < end; i += kThreads) x[i] = (m ? update_of(g[i], m[i], mu, nesterov) : g[i]) * inverse;
+    for (long long i = base + threadIdx.x; i < end; i += kThreads) x[i] = (m ? update_of(g[i], m[i], mu, nesterov) : g[i]) * inverse.first * inverse.second;
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -140,7 +147,8 @@ muon_planes_kernel(const __grid_constant__ List list, float mu, bool nesterov, f
     grid_dependency_trigger();
     grid_dependency_wait();
     const int t = find(list, blockIdx.x), rows = list.rows[t], cols = list.cols[t];
-    const float factor = inverse_norm(list, t, partial, eps, red) * scale;
+    const Inverse inverse = inverse_norm(list, t, partial, eps, red);
+    const float first = inverse.first, second = inverse.second * scale;
     const float *const m = list.momentum[t], *const g = list.grad[t];
     uint16_t *const dst = list.planes[t];
     const FastDiv per_row = list.vectors[t];
@@ -173,7 +181,7 @@ muon_planes_kernel(const __grid_constant__ List list, float mu, bool nesterov, f
         unsigned *const h = &hi.x, *const l = &lo.x;
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            const float a = (m ? update_of(x[i], y[i], mu, nesterov) : x[i]) * factor, b = (m ? update_of(x[i + 1], y[i + 1], mu, nesterov) : x[i + 1]) * factor;
+            const float a = (m ? update_of(x[i], y[i], mu, nesterov) : x[i]) * first * second, b = (m ? update_of(x[i + 1], y[i + 1], mu, nesterov) : x[i + 1]) * first * second;
             const __half2 top = __floats2half2_rn(a, b);
             const float2 back = __half22float2(top);
             constexpr float up = 1 << kHalfLoShift;

@@ -62,6 +62,42 @@ def test_orthogonalize(F, shape):
     close(got.torch_view(), *truth(g))
 
 
+def test_more_matrices_than_a_launch_takes(F):
+    g = gradient(5, 700, 12, 9)
+    got = F.orthogonalize(tensor(F, g)).torch_view()
+    F.device_status()
+    close(got, *truth(g))
+
+
+def test_more_shapes_than_a_launch_takes(F):
+    """Shapes of one launch run side by side, long and short, tall and wide."""
+    shapes = [(16 + 24 * i, 300 - 23 * i) for i in range(12)] + [(64, 700), (900, 40)]
+    ps, ms, gs = ([gradient(7 * i + j, *s) for i, s in enumerate(shapes)] for j in range(3))
+    want = [step_truth(p, m, g, 0.05, 0.95, True, 0.0, 0.5) for p, m, g in zip(ps, ms, gs)]
+    F.muon_step([tensor(F, t) for t in ps], [tensor(F, t) for t in ms], [tensor(F, t) for t in gs], lr=0.05, scale=0.5)
+    F.device_status()
+    for p, (wp, _, off) in zip(ps, want):
+        assert torch.linalg.matrix_norm(p.double() - wp) <= off + 2.0 ** -23 * torch.linalg.matrix_norm(wp)
+
+
+def test_two_streams_in_turn(F):
+    """Calls on two streams, ordered by events as the scratch of a device asks for."""
+    shapes = [(300, 500), (512, 128), (300, 500)]
+    ps, ms, gs = ([gradient(11 * i + j, *s) for i, s in enumerate(shapes)] for j in range(3))
+    qs, ns = ([t.clone() for t in ts] for ts in (ps, ms))
+    for _ in range(4):
+        F.muon_step([tensor(F, t) for t in qs], [tensor(F, t) for t in ns], [tensor(F, t) for t in gs], lr=0.05)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for k in range(4):
+        streams[k % 2].wait_stream(streams[1 - k % 2])
+        with torch.cuda.stream(streams[k % 2]):
+            F.muon_step([tensor(F, t) for t in ps], [tensor(F, t) for t in ms], [tensor(F, t) for t in gs], lr=0.05)
+    torch.cuda.synchronize()
+    F.device_status()
+    assert all(torch.equal(a, b) for a, b in zip(ps + ms, qs + ns))
+
+
 def test_singular_values_are_nearly_one(F):
     gen = torch.Generator(device="cuda").manual_seed(3)
     g = torch.randn(200, 600, device="cuda", generator=gen)
@@ -75,6 +111,18 @@ def test_any_size_of_gradient(F, scale, shape):
     g = gradient(4, *shape) * scale
     got = F.orthogonalize(tensor(F, g), eps=0.0)
     close(got.torch_view(), *truth(g, eps=0.0))
+
+
+@pytest.mark.parametrize("steps", [0, 5])
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -138, 2.0 ** 127])
+def test_norms_beyond_the_normal_range(F, scale, steps):
+    """Elements of 8 bits times a power of two, exact where f32 has subnormals only; the norm's inverse, or the norm, is beyond f32's normal range."""
+    g = torch.round(gradient(4, 40, 24) * 1e5).clamp(-127, 127) * 2.0 ** -7
+    h = (g.double() * scale).float()
+    assert torch.equal(h.double(), g.double() * scale)
+    got = F.orthogonalize(tensor(F, h), steps=steps, eps=0.0).torch_view()
+    want, off = truth(g, steps, eps=0.0)
+    assert torch.isfinite(got).all() and torch.linalg.matrix_norm(got.double() - want) <= off
 
 
 @pytest.mark.parametrize("steps", [0, 1, 3, 9])
