@@ -20,14 +20,21 @@
 // that lies below is loaded from above and given to the tensor core as what it is, MN-major.
 //
 // Tiles: 256 x 256 of a pair (24.4 clocks an element of the contraction: the pipe's 24), 128 x 128 of a lone CTA (24: its shared memory
-// feeds half of the pipe) or 128 x 64 (15).  The smaller ones have less to do in the chain of a single matrix, the large ones do twice as
-// much a clock: tiling() weighs the two.
+// feeds half of the pipe) or 128 x 64 (15, 20 with its operands from L2).  The smaller ones have less to do in the chain of a single matrix,
+// the large ones do twice as much a clock: tiling() weighs the two.
+//
+// What bounds it.  One matrix: the chain of 15 products, each of which takes its contraction (16000 clocks at 768), 1200 for the first operands,
+// 700 for the accumulators, 2500 for the planes, 1500 until they are counted and 2000 until the others see that; 768 x 768 takes 203 us,
+// 64 x 32 68.  Many: thirty matrices of 512 x 512 and 512 x 2048 take 725 us, the pipe busy for 45 %, L2 at 8.1 TB/s, 1.2 GB from and to DRAM (their planes
+// are 220 MB, more than L2 holds): a tile of 512 elements takes 12500 clocks of the pipe and 10000 of its epilogue, during which the next tile's
+// accumulators can only fill once.
 #include "fused_epilogue.h"
 #include "internal.h"
 #include "tcgen05.h"
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 
 namespace mni {
@@ -576,10 +583,10 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
 // ------------------------------------------------------------------ host side
 struct Tiling {
     int bn, cg;
-    double clocks_k, round;        // of a unit: per contraction element, and beside its main loop where units follow one another
+    double clocks_k, round;        // of a unit: per contraction element (with operands from L2), and beside its main loop where units follow one another
     double chain;                  // of a product in the chain of one matrix: count, first operands, epilogue
 };
-constexpr Tiling kTilings[] = {{256, 2, 24.4, 1500, 11000}, {128, 1, 24.0, 1500, 8500}, {64, 1, 15.0, 1200, 6500}};
+constexpr Tiling kTilings[] = {{256, 2, 24.4, 8000, 17000}, {128, 1, 24.0, 5000, 9500}, {64, 1, 20.0, 3000, 9500}};
 
 int64_t symmetric_tiles(int64_t side, int tm, int bn) {
     const int64_t m = (side + tm - 1) / tm, n = (side + bn - 1) / bn, ratio = tm / bn;
@@ -588,7 +595,10 @@ int64_t symmetric_tiles(int64_t side, int tm, int bn) {
     return tiles;
 }
 
-// The tiling whose estimate is least: the slots' share of all units, or the chain of the longest matrix, whichever is more.
+// The tiling whose estimate is least: the rounds of all units, or the chain of the longest matrix, whichever is more, and some of the other.
+// us with tiles of 64 / 128 / 256 columns: one matrix of 256 x 256 118 / 144 / 203, 768 206 / 241 / 303, 1024 258 / 294 / 356, 1536 639 / 414 /
+// 469, 2048 1071 / 670 / 614; three of 1001 x 333 182 / 215 / 271; twenty of 512 x 512 and ten of 512 x 2048 and turned 1130 / 839 / 736; six of
+// 2048 x 2048 to 2048 x 8192 10000 / 7020 / 5180.
 const Tiling &tiling(const NewtonProblem *g, int count, int sm_count) {
     const int env = env_int("MNI_B200_NEWTON_TILE", 0);
     const Tiling *best = nullptr;
@@ -596,16 +606,20 @@ const Tiling &tiling(const NewtonProblem *g, int count, int sm_count) {
     for (const Tiling &t : kTilings) {
         if (env == t.bn) return t;
         const int tm = BM * t.cg;
+        const double slots = std::max(1, sm_count / t.cg);
         double work = 0, chain = 0;
         for (int i = 0; i < count; ++i) {
             const double side = static_cast<double>(g[i].side()), longer = static_cast<double>(std::max(g[i].rows, g[i].cols));
             const double t1 = static_cast<double>(symmetric_tiles(g[i].side(), tm, t.bn)),
                          t3 = static_cast<double>((g[i].rows + tm - 1) / tm) * static_cast<double>((g[i].cols + t.bn - 1) / t.bn);
-            auto unit = [&](double k) { return std::max(t.clocks_k * std::max(k, 64.0) + t.round, 0.45 * t.chain); };
-            work += g[i].count * (t1 * (unit(longer) + unit(side)) + t3 * unit(side));
+            auto unit = [&](double k) { return t.clocks_k * std::max(k, 64.0) + t.round; };
+            // (products of several shapes fill each other's last round)
+            auto rounds = [&](double units) { return count == 1 ? std::ceil(units / slots) : units / slots; };
+            const double n = static_cast<double>(g[i].count);
+            work += rounds(t1 * n) * (unit(longer) + unit(side)) + rounds(t3 * n) * unit(side);
             chain = std::max(chain, t.clocks_k * (longer + 2 * side) + 3 * t.chain);
         }
-        const double slots = std::max(1, sm_count / t.cg), time = std::max(work / slots, chain) + 0.3 * std::min(work / slots, chain);
+        const double time = std::max(work, chain) + 0.3 * std::min(work, chain);
         if (time < least) {
             least = time;
             best = &t;
