@@ -62,6 +62,23 @@ def test_orthogonalize(F, shape):
     close(got.torch_view(), *truth(g))
 
 
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+@pytest.mark.parametrize("shape", [(1, 1), (40, 70), (257, 130), (300, 300), (700, 333), (520, 1030), (3, 257, 513)])
+def test_every_tiling(F, monkeypatch, tile, shape):
+    """Tiles that one matrix of these sizes would not be given: ragged ones, and blocks below the diagonal read from above."""
+    monkeypatch.setenv("MNI_B200_NEWTON_TILE", tile)
+    g = gradient(sum(shape), *shape)
+    got = F.orthogonalize(tensor(F, g)).torch_view()
+    F.device_status()
+    close(got, *truth(g))
+    batch = (shape[0],) if len(shape) == 3 else ()
+    p, m, u = (gradient(9 + i, *batch, *shape[-2:]) for i in range(3))
+    want, _, off = step_truth(p, m, u, 0.05, 0.95, True, 0.02, 0.5)
+    F.muon_step([tensor(F, p)], [tensor(F, m)], [tensor(F, u)], lr=0.05, weight_decay=0.02, scale=0.5)
+    F.device_status()
+    assert (torch.linalg.matrix_norm(p.double() - want) <= off + 2.0 ** -23 * torch.linalg.matrix_norm(want)).all()
+
+
 def test_more_matrices_than_a_launch_takes(F):
     g = gradient(5, 700, 12, 9)
     got = F.orthogonalize(tensor(F, g)).torch_view()
