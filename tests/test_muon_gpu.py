@@ -292,3 +292,22 @@ def test_the_step_that_training_takes(F):
     wp, wm, off = step_truth(before, torch.zeros_like(w), dw.torch_view(), 0.02, 0.95, True, 0.01, (700 / 96) ** 0.5)
     assert torch.linalg.matrix_norm(w.double() - wp) <= off + 2.0 ** -23 * torch.linalg.matrix_norm(wp)
     assert ((m.double() - wm).abs() <= 2.0 ** -23 * wm.abs()).all()
+
+
+@pytest.mark.parametrize("tile", ["64", "256"])
+def test_wait_limit_runs_out_then_the_library_recovers(F, monkeypatch, tile):
+    """Copies of one stage that the test hook withholds: every role's wait ends, the status says so, and the next call is right."""
+    g = gradient(8, 300, 280)
+    assert F.device_status() == 0
+    monkeypatch.setenv("MNI_B200_NEWTON_TILE", tile)
+    monkeypatch.setenv("MNI_B200_WAIT_CYCLES", "2000000")           # about 1 ms
+    monkeypatch.setenv("MNI_B200_TEST_WITHHOLD_KBLOCK", "3")
+    F.orthogonalize(tensor(F, g))
+    with pytest.raises(F._lib.MniError) as ei:
+        F.device_status()
+    assert ei.value.status == 8 and "bounded wait" in ei.value.message
+    monkeypatch.delenv("MNI_B200_TEST_WITHHOLD_KBLOCK")
+    monkeypatch.delenv("MNI_B200_WAIT_CYCLES")
+    assert F.device_status() == 0
+    close(F.orthogonalize(tensor(F, g)).torch_view(), *truth(g))
+    assert F.device_status() == 0
