@@ -1574,7 +1574,7 @@ int loss_bwd_planes(Call &c, const LossCall &l, const float *lse, const float *g
             p[n].accumulate = (flags & MNI_B200_ACCUMULATE_DB) != 0;
             ++n;
         }
-        for (int i = 0; i < n; ++i) p[i].chunk_k = env_int("MNI_B200_DRAIN_K", kLossChunkK);
+        for (int i = 0; i < n; ++i) p[i].chunk_k = kLossChunkK;
         if (n) rc = run_halves(c, p, n, h, a, b, nullptr);
         if (rc == MNI_B200_OK && dbias) {
             const size_t part = c.arena.reserve(grad_column_sums_bytes(l.M, count, c.st->sm_count));

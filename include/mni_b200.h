@@ -232,6 +232,10 @@ MNI_B200_API int mni_b200_clip_and_step(int64_t count, float *const *params, flo
  * whatever its row of x holds.  One of N or more makes the row's loss NaN, and with it the gradients.
  * `reduction`: NONE leaves M losses in `loss`; SUM and MEAN one number, MEAN over the rows that are not left out (NaN where there
  * is none).  `lse` takes M numbers (those of rows left out too), which the backward needs.
+ *
+ * Scratch, which mni_b200_workspace_query does not cover: 6 bytes an element of x and w and a pair (8 bytes) for every row and 64 classes; the
+ * backward 6 bytes an element of x, w and a copy of x, that copy, dx once more, and 6 bytes a logit of as many classes as 384 MB hold.  Calls of up to 8
+ * rows, or up to 2^23 multiply-adds, 4 bytes a logit.  A captured call is run once beforehand, as any other that cannot do without.
  */
 #define MNI_B200_REDUCE_NONE 0
 #define MNI_B200_REDUCE_SUM  1
@@ -265,6 +269,9 @@ MNI_B200_API int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int 
  *   param = (1 - lr * weight_decay) * param - lr * scales[i] * orthogonalize(u)
  * params and momenta are updated in place, grads are read; no two of an entry's three may share memory.  Entries that share memory with
  * others are stepped one after the other, in list order.  (No counterpart in the reference.)
+ *
+ * Scratch of both, which mni_b200_workspace_query does not cover: 8 bytes an element of a matrix and 12 of its smaller side squared, rows padded to
+ * 64 elements, for as many matrices as 2 GB hold, one at least.
  */
 MNI_B200_API int mni_b200_muon_step(int64_t count, float *const *params, float *const *momenta, const float *const *grads,
                                     const int64_t *rows, const int64_t *cols, const float *scales, float lr, float momentum,

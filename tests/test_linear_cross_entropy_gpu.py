@@ -116,6 +116,23 @@ def test_loss_and_gradients(F, rows, k, n, layout):
     compare(F, x, w, t, b)
 
 
+@pytest.mark.parametrize("piece", ["256", "768"])
+@pytest.mark.parametrize("lone", ["0", "1"])
+@pytest.mark.parametrize("layout", ["stored", "tied"])
+@pytest.mark.parametrize("rows,k,n", [(300, 200, 1000), (257, 130, 2049)])
+def test_pieces_of_the_classes(F, monkeypatch, piece, lone, layout, rows, k, n):
+    """The backward in pieces, the last one ragged, as many classes and rows make it; with tiles of pairs and of single CTAs."""
+    monkeypatch.setenv("MNI_B200_LOSS_PIECE", piece)
+    monkeypatch.setenv("MNI_B200_FUSED_LONE", lone)
+    compare(F, *make(rows + n, rows, k, n, layout, bias=True, masked=True, spread=2.0))
+
+
+@pytest.mark.parametrize("rows,k,n", [(4096, 8, 12), (4097, 8, 12), (50, 64, 128), (50, 65, 129), (30, 250, 30), (30, 260, 30), (20, 8, 1024), (20, 9, 1025)])
+def test_few_short_rows(F, rows, k, n):
+    """Both sides of the limits of the kernel that makes logits and what becomes of them in one launch."""
+    compare(F, *make(rows + k, rows, k, n, bias=True, masked=True))
+
+
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("rows,k,n", [(5, 32, 100), (70, 48, 333), (600, 128, 1500)])
 def test_reductions(F, reduction, rows, k, n):
