@@ -1890,6 +1890,14 @@ int env_int(const char *name, int dflt) {
     return v ? atoi(v) : dflt;
 }
 
+cudaError_t check_launch_registers(const void *kernel, int planned) {
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, kernel);
+    if (e != cudaSuccess) return e;
+    // test hook: stands in for what the compiler gave, if that is more
+    return std::min(f.numRegs, env_int("MNI_B200_TEST_LAUNCH_REGS", f.numRegs)) < planned ? cudaErrorInvalidConfiguration : cudaSuccess;
+}
+
 int fail(int status, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);

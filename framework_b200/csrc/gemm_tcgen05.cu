@@ -347,6 +347,12 @@ struct RegShare {
 // ... and of the two-accumulator variant, 168 of 384 threads at launch: two epilogue warpgroups and the one of all other roles.
 constexpr int kTwoEpilogue = 224, kTwoIssue = 56, kTwoLaunch = 168;
 static_assert(2 * kTwoEpilogue + kTwoIssue <= 3 * kTwoLaunch, "more registers than the launch has");
+// Registers a thread that a variant's shares count on at launch; 0 where warps keep what they have.
+template <int MODE, int TAIL>
+constexpr int planned_registers() {
+    if (MODE == kHalfThree || MODE == kHalfDrain) return kTwoLaunch;
+    return TAIL == kRunningSum ? RegShare<MODE>::kLaunch : 0;
+}
 __host__ __device__ constexpr int product_slots(int mode, int tail) { return (mode == kHalfThree || mode == kHalfOne || mode == kHalfDrain) && !is_fused(tail) ? 2 : 1; }
 template <int MODE, int TAIL>
 using KernelArgs = std::conditional_t<is_fused(TAIL), FusedProduct, Products<product_slots(MODE, TAIL)>>;
@@ -2180,6 +2186,10 @@ cudaError_t launch_variant(const Plan &pl, const Product *const *w, int count, c
         attr = cudaFuncSetAttribute(gemm_tc_kernel<BN, BK, MODE, NS, CG, TA, TAIL, SG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     227 * 1024);
         if (attr != cudaSuccess) return attr;
+        if constexpr (planned_registers<MODE, TAIL>() > 0) {
+            attr = check_launch_registers(reinterpret_cast<const void *>(gemm_tc_kernel<BN, BK, MODE, NS, CG, TA, TAIL, SG>), planned_registers<MODE, TAIL>());
+            if (attr != cudaSuccess) return attr;
+        }
         opted_in.fetch_or(bit, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg{};

@@ -93,6 +93,9 @@ struct EnvScope {
 const char *env_value(const char *name);              // value, or nullptr if unset or empty
 int env_int(const char *name, int dflt);
 int device_sm_count();                                // SM count of the current device (cached per device)
+// Whether the compiler gave a kernel at least `planned` registers a thread, which is what its shares of setmaxnreg add up to: of a launch with
+// fewer setmaxnreg.inc waits for good, and no limit of ours ends that.  Asked once per kernel and device, before its first launch.
+cudaError_t check_launch_registers(const void *kernel, int planned);
 extern std::atomic<uint64_t> g_launches;              // kernels launched by this library
 
 #define MNI_CUDA(call)                                                                   \

@@ -44,7 +44,7 @@ namespace {
 constexpr int BM = 128, BK = 64, kStagesMax = 8, kEpiWarps = 8, kPatchBytes = 4096, kRing = 2;
 constexpr int kPieceBlocks = 2;                    // k-blocks whose large terms share an accumulator's chain: 128 elements
 constexpr int kThreads = 32 * (4 + kEpiWarps);
-constexpr int kLaunchRegs = 168;                   // a thread has at launch; launch() checks that the compiler took as many
+constexpr int kLaunchRegs = 168;                   // a thread has at launch; launch() checks that the compiler took no fewer
 constexpr int kIssueRegs = 56, kEpiRegs = 224;
 static_assert(kThreads * kLaunchRegs <= 65536 && kIssueRegs + 2 * kEpiRegs <= 3 * kLaunchRegs, "more registers than the launch has");
 constexpr int kBars = 3 * kStagesMax + 4 + 2 * kRing + 1;
@@ -639,10 +639,8 @@ cudaError_t launch(const Args &args, int units, size_t smem, int sm_count, cudaS
     if ((opted_in.load(std::memory_order_acquire) & bit) == 0) {
         e = cudaFuncSetAttribute(newton_schulz_kernel<BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
         if (e != cudaSuccess) return e;
-        cudaFuncAttributes f;                      // setmaxnreg.inc beyond what the launch has would wait for good
-        e = cudaFuncGetAttributes(&f, newton_schulz_kernel<BN, CG>);
+        e = check_launch_registers(reinterpret_cast<const void *>(newton_schulz_kernel<BN, CG>), kLaunchRegs);
         if (e != cudaSuccess) return e;
-        if (f.numRegs != kLaunchRegs) return cudaErrorInvalidConfiguration;
         opted_in.fetch_or(bit, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg{};
