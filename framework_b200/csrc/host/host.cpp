@@ -859,6 +859,18 @@ PyObject *op_clip_and_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     return PyFloat_FromDouble(static_cast<double>(norm));
 }
 
+// Whether a tensor (null or None: nothing to ask) is where the others of a call are: kernels take plain pointers.
+bool on_device(const TensorObj *t, const at::Device &device, const char *what) {
+    if (!t || t->flat.device() == device) return true;
+    PyErr_Format(PyExc_ValueError, "%s is on %s, the call's other tensors are on %s", what, t->flat.device().str().c_str(), device.str().c_str());
+    return false;
+}
+bool given_on_device(PyObject *o, const at::Device &device, const char *what) {
+    if (o == Py_None) return true;
+    const TensorObj *t = as_tensor(o, what);
+    return t && on_device(t, device, what);
+}
+
 // ------------------------------------------------------------------ cross entropy of a projection
 // What the two operators check alike: x [.., K], weight [K, N], whole-number targets of x's leading shape, bias [N] or None.
 struct LossOperands {
@@ -900,6 +912,7 @@ struct LossOperands {
             bias = as_tensor(pb, "bias");
             if (!bias) return false;
             if (!vector_of(bias, n) || !bias->contiguous) { PyErr_SetString(PyExc_ValueError, "bias must be a contiguous [N] vector"); return false; }
+            if (!on_device(bias, x->flat.device(), "bias")) return false;
         }
         reduction = static_cast<int>(PyLong_AsLong(pr));
         return !PyErr_Occurred();
@@ -940,9 +953,12 @@ PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py
         PyErr_SetString(PyExc_ValueError, "grad must have the loss's shape");
         return nullptr;
     }
+    const at::Device device = o.x->flat.device();
+    if (!on_device(g0, device, "grad") || !on_device(s0, device, "lse") || (need_dx && !given_on_device(args[11], device, "dx")) ||
+        (need_dw && !given_on_device(args[12], device, "dw")) || (want_dbias && !given_on_device(args[13], device, "dbias")))
+        return nullptr;
     Ref g(contiguous_of(g0)), lse(g ? contiguous_of(s0) : nullptr);
     if (!g || !lse) return nullptr;
-    const at::Device device = o.x->flat.device();
     Ref dx, dw, dbias;
     if (need_dx && !output(args[11], o.x->shape, device, "dx", dx)) return nullptr;
     // a weight seen through a transposing view has its gradient laid out as it is stored itself
@@ -1041,12 +1057,15 @@ PyObject *op_muon_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     std::vector<const float *> g;
     std::vector<int64_t> rows, cols;
     std::vector<float> scales;
+    at::Device device(at::kCUDA);                  // the first parameter's
     for (Py_ssize_t i = 0; i < count; ++i) {
         TensorObj *t[3];
         for (int k = 0; k < 3; ++k) {
             t[k] = as_tensor(PySequence_Fast_GET_ITEM(lists[k], i), "every element");
             if (!t[k]) return nullptr;
             if (!t[k]->contiguous) { PyErr_SetString(PyExc_ValueError, "muon_step needs contiguous tensors"); return nullptr; }
+            if (i == 0 && k == 0) device = t[0]->flat.device();
+            if (!on_device(t[k], device, "an element")) return nullptr;
         }
         const Dims &shape = t[0]->shape;
         if (t[1]->shape != shape || t[2]->shape != shape) {

@@ -1,0 +1,47 @@
+"""CPU: what the operators refuse on the host, for tensors that have a device and a shape and no memory."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+X, W, ROWS = (6, 8), (8, 10), (6,)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    from framework_b200 import build
+    build.build_library()
+
+
+def flat(n, device="cuda:0", dtype=torch.float32):
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        return torch.empty(n, device=device, dtype=dtype)
+
+
+def tensor(shape, device="cuda:0", strides=None):
+    from framework_b200 import DeviceTensor
+    n = 1
+    for s in shape:
+        n *= s
+    return DeviceTensor(flat(n, device), shape, strides)
+
+
+def targets():
+    return flat(6, dtype=torch.int64)
+
+
+def test_every_tensor_of_a_call_is_on_one_device():
+    """Those of another GPU would reach the kernels as plain pointers."""
+    from framework_b200 import ops
+    there = "cuda:1"
+    with pytest.raises(ValueError, match="bias is on cuda:1.*cuda:0"):
+        ops.linear_cross_entropy(tensor(X), tensor(W), targets(), tensor((10,), there))
+    good = dict(grad=tensor((1,)), x=tensor(X), weight=tensor(W), targets=targets(), lse=tensor(ROWS))
+    for name, value in [("grad", tensor((1,), there)), ("lse", tensor(ROWS, there)), ("bias", tensor((10,), there)), ("dx", tensor(X, there)),
+                        ("dw", tensor(W, there)), ("dw", tensor((10, 8), there).permute([1, 0])), ("dbias", tensor((10,), there))]:
+        with pytest.raises(ValueError, match=f"{name} is on cuda:1"):
+            ops.linear_cross_entropy_backward(**{**good, name: value}, want_dbias=True)
+    for which in range(6):
+        lists = [[tensor((4, 5)), tensor((4, 5))] for _ in range(3)]
+        lists[which // 2][which % 2] = tensor((4, 5), there)
+        with pytest.raises(ValueError, match="on cuda"):
+            ops.muon_step(*lists, lr=0.1)
