@@ -871,6 +871,14 @@ bool given_on_device(PyObject *o, const at::Device &device, const char *what) {
     return t && on_device(t, device, what);
 }
 
+// ... and whether that is the device whose stream the call's kernels go to.
+bool on_current_device(const at::Device &device) {
+    const int current = c10::cuda::current_device();
+    if (device.index() == current) return true;
+    PyErr_Format(PyExc_ValueError, "the tensors are on %s, the current device is cuda:%d", device.str().c_str(), current);
+    return false;
+}
+
 // ------------------------------------------------------------------ cross entropy of a projection
 // What the two operators check alike: x [.., K], weight [K, N], whole-number targets of x's leading shape, bias [N] or None.
 struct LossOperands {
@@ -925,6 +933,7 @@ PyObject *op_linear_cross_entropy(PyObject *, PyObject *const *args, Py_ssize_t 
     LossOperands o;
     if (!o.parse(args[0], args[1], args[2], args[3], args[4])) return nullptr;
     const at::Device device = o.x->flat.device();
+    if (!on_current_device(device)) return nullptr;
     Ref loss(new_tensor(o.reduction == MNI_B200_REDUCE_NONE ? o.rows : Dims{1}, device)), lse(loss ? new_tensor(o.rows, device) : nullptr);
     if (!loss || !lse) return nullptr;
     mni_b200_view vx, vw;
@@ -955,7 +964,8 @@ PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py
     }
     const at::Device device = o.x->flat.device();
     if (!on_device(g0, device, "grad") || !on_device(s0, device, "lse") || (need_dx && !given_on_device(args[11], device, "dx")) ||
-        (need_dw && !given_on_device(args[12], device, "dw")) || (want_dbias && !given_on_device(args[13], device, "dbias")))
+        (need_dw && !given_on_device(args[12], device, "dw")) || (want_dbias && !given_on_device(args[13], device, "dbias")) ||
+        !on_current_device(device))
         return nullptr;
     Ref g(contiguous_of(g0)), lse(g ? contiguous_of(s0) : nullptr);
     if (!g || !lse) return nullptr;
@@ -1018,6 +1028,7 @@ PyObject *op_orthogonalize(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     NewtonSchulzArgs ns;
     if (!ns.parse(args + 1)) return nullptr;
     if (g->shape.size() < 2) { PyErr_SetString(PyExc_ValueError, "orthogonalize requires at least 2D tensors"); return nullptr; }
+    if (!on_current_device(g->flat.device())) return nullptr;
     Ref out(new_tensor(g->shape, g->flat.device()));
     if (!out) return nullptr;
     mni_b200_view vg;
@@ -1058,14 +1069,19 @@ PyObject *op_muon_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     std::vector<int64_t> rows, cols;
     std::vector<float> scales;
     at::Device device(at::kCUDA);                  // the first parameter's
+    for (Py_ssize_t i = 0; i < 3 * count; ++i) {
+        const TensorObj *t = as_tensor(PySequence_Fast_GET_ITEM(lists[i % 3], i / 3), "every element");
+        if (!t) return nullptr;
+        if (i == 0) device = t->flat.device();
+        if (!on_device(t, device, "an element")) return nullptr;
+    }
+    if (count > 0 && !on_current_device(device)) return nullptr;
     for (Py_ssize_t i = 0; i < count; ++i) {
         TensorObj *t[3];
         for (int k = 0; k < 3; ++k) {
             t[k] = as_tensor(PySequence_Fast_GET_ITEM(lists[k], i), "every element");
             if (!t[k]) return nullptr;
             if (!t[k]->contiguous) { PyErr_SetString(PyExc_ValueError, "muon_step needs contiguous tensors"); return nullptr; }
-            if (i == 0 && k == 0) device = t[0]->flat.device();
-            if (!on_device(t[k], device, "an element")) return nullptr;
         }
         const Dims &shape = t[0]->shape;
         if (t[1]->shape != shape || t[2]->shape != shape) {

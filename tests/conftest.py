@@ -92,3 +92,13 @@ def regression_bound_3xtf32(k):
     accumulation rounding, which grows like sqrt(K) * 2^-24.  A single-pass TF32 product sits near 3e-4,
     two orders of magnitude above this at every K the tests use, so a broken split cannot hide under it."""
     return 5e-6 + 1.2e-7 * float(np.sqrt(max(int(k), 1)))
+
+
+def fake_cuda(n, device, dtype=None):
+    """A flat torch tensor that says it is on a CUDA device, whether there is one or not, and has no memory: for what the host refuses."""
+    from unittest import mock
+
+    import torch
+    from torch._subclasses import fake_tensor
+    with mock.patch.object(fake_tensor, "init_gpu_context", lambda *_: None), fake_tensor.FakeTensorMode(allow_non_fake_inputs=True):
+        return torch.empty(n, device=device, dtype=dtype or torch.float32)

@@ -1,7 +1,8 @@
 """CPU: what the operators refuse on the host, for tensors that have a device and a shape and no memory."""
 import pytest
 import torch
-from torch._subclasses.fake_tensor import FakeTensorMode
+
+from conftest import fake_cuda
 
 X, W, ROWS = (6, 8), (8, 10), (6,)
 
@@ -12,21 +13,16 @@ def library():
     build.build_library()
 
 
-def flat(n, device="cuda:0", dtype=torch.float32):
-    with FakeTensorMode(allow_non_fake_inputs=True):
-        return torch.empty(n, device=device, dtype=dtype)
-
-
 def tensor(shape, device="cuda:0", strides=None):
     from framework_b200 import DeviceTensor
     n = 1
     for s in shape:
         n *= s
-    return DeviceTensor(flat(n, device), shape, strides)
+    return DeviceTensor(fake_cuda(n, device), shape, strides)
 
 
 def targets():
-    return flat(6, dtype=torch.int64)
+    return fake_cuda(6, "cuda:0", torch.int64)
 
 
 def test_every_tensor_of_a_call_is_on_one_device():
