@@ -953,6 +953,16 @@ PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py
     bool need_dx, need_dw, want_dbias;
     if (!parse_flags(args[7], flags) || !parse_truth(args[8], need_dx) || !parse_truth(args[9], need_dw) || !parse_truth(args[10], want_dbias))
         return nullptr;
+    const struct {
+        uint32_t flag;
+        bool wanted;
+        const char *name;
+    } added[3] = {{MNI_B200_ACCUMULATE_DA, need_dx, "dx"}, {MNI_B200_ACCUMULATE_DB, need_dw, "dw"}, {MNI_B200_ACCUMULATE_DBIAS, want_dbias, "dbias"}};
+    for (int i = 0; i < 3; ++i)
+        if ((flags & added[i].flag) != 0 && added[i].wanted && args[11 + i] == Py_None) {
+            PyErr_Format(PyExc_ValueError, "flags add to %s, and none is given", added[i].name);
+            return nullptr;
+        }
     LossOperands o;
     if (!o.parse(args[1], args[2], args[3], args[5], args[6])) return nullptr;
     TENSOR(g0, 0, "grad");

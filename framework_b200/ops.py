@@ -156,7 +156,7 @@ def linear_cross_entropy_backward(grad: DeviceTensor, x: DeviceTensor, weight: D
     """Backward of ``linear_cross_entropy`` -> (dx, dw[, dbias]); ``grad`` has the loss's shape.
 
     ``dw`` has the weight's shape; it is laid out as the weight is stored, so the gradient of a transposing view of a stored [N, K] is such a
-    view itself.  With the ACCUMULATE flags the gradients are added to the ``dx``, ``dw``, ``dbias`` given."""
+    view itself.  With the ACCUMULATE flags the gradients are added to the ``dx``, ``dw``, ``dbias`` given, which have to be."""
     return _host.linear_cross_entropy_backward(grad, x, weight, targets, lse, bias, _reduction(reduction), flags, need_dx, need_dw,
                                                want_dbias, dx, dw, dbias)
 

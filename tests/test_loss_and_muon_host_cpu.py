@@ -41,3 +41,11 @@ def test_every_tensor_of_a_call_is_on_one_device():
         lists[which // 2][which % 2] = tensor((4, 5), there)
         with pytest.raises(ValueError, match="on cuda"):
             ops.muon_step(*lists, lr=0.1)
+
+
+@pytest.mark.parametrize("flag,wanted", [("ACCUMULATE_DA", "dx"), ("ACCUMULATE_DB", "dw"), ("ACCUMULATE_DBIAS", "dbias")])
+def test_nothing_is_added_to_memory_that_was_not_given(flag, wanted):
+    """A gradient that the call allocates itself holds whatever was there before."""
+    from framework_b200 import _lib, ops
+    with pytest.raises(ValueError, match=f"flags add to {wanted}, and none is given"):
+        ops.linear_cross_entropy_backward(tensor((1,)), tensor(X), tensor(W), targets(), tensor(ROWS), flags=getattr(_lib, flag), want_dbias=True)
