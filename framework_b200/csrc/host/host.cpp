@@ -953,6 +953,7 @@ PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py
     bool need_dx, need_dw, want_dbias;
     if (!parse_flags(args[7], flags) || !parse_truth(args[8], need_dx) || !parse_truth(args[9], need_dw) || !parse_truth(args[10], want_dbias))
         return nullptr;
+    flags &= ~MNI_B200_DB_TRANSPOSED;              // a matter of dw's strides alone
     const struct {
         uint32_t flag;
         bool wanted;

@@ -25,3 +25,22 @@ def test_another_device_than_the_current_one_is_refused(F):
         with pytest.raises(ValueError, match=f"the tensors are on {there}, the current device is"):
             call()
     assert F.launch_count() == before
+
+
+@pytest.mark.parametrize("rows", [6, 300])
+@pytest.mark.parametrize("layout", ["stored", "tied"])
+def test_the_layout_of_dw_is_its_strides(F, rows, layout):
+    """The C interface's flag for a turned dw says nothing here, where dw's strides say it."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, 64, device="cuda", generator=gen)
+    w = torch.randn(64, 500, device="cuda", generator=gen) if layout == "stored" else torch.randn(500, 64, device="cuda", generator=gen).t()
+    t = torch.randint(0, 500, (rows,), device="cuda", generator=gen)
+    one = tensor(F, torch.ones(1, device="cuda"))
+    _, lse = F.linear_cross_entropy(tensor(F, x), tensor(F, w), t)
+    want = F.linear_cross_entropy_backward(one, tensor(F, x), tensor(F, w), t, lse)
+    for dw in (None, tensor(F, torch.empty(64, 500, device="cuda")), tensor(F, torch.empty(500, 64, device="cuda").t())):
+        got = F.linear_cross_entropy_backward(one, tensor(F, x), tensor(F, w), t, lse, flags=F._lib.DB_TRANSPOSED, dw=dw)
+        F.device_status()
+        assert got[1].shape == (64, 500)
+        # (of either layout the sums are the same up to their order: 300 terms)
+        assert float((got[1].torch_view() - want[1].torch_view()).abs().max()) <= 1e-5 * float(want[1].torch_view().abs().max())
