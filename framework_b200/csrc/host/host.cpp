@@ -984,7 +984,7 @@ PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py
     if (need_dx && !output(args[11], o.x->shape, device, "dx", dx)) return nullptr;
     // a weight seen through a transposing view has its gradient laid out as it is stored itself
     const Dims shape{o.k, o.n}, stored{o.n, o.k};
-    bool turned = o.k > 1 && o.n > 1 && o.w->stride[0] == 1 && o.w->stride[1] != 1;
+    bool turned = o.k > 1 && o.n > 1 && o.w->stride.size() == 2 && o.w->stride[0] == 1 && o.w->stride[1] != 1;
     if (need_dw && args[12] == Py_None) {
         dw.reset(new_tensor(turned ? stored : shape, device));
         if (dw && turned) dw.reset(reinterpret_cast<TensorObj *>(permuted(dw.t, Dims{1, 0})));
@@ -995,7 +995,7 @@ PyObject *op_linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py
     }
     if (want_dbias && !output(args[13], Dims{o.n}, device, "dbias", dbias)) return nullptr;
     if ((dx && (dx.t->shape != o.x->shape || !dx.t->contiguous)) || (dbias && (!vector_of(dbias.t, o.n) || !dbias.t->contiguous)) ||
-        (dw && (dw.t->shape != shape || (turned && !(dw.t->stride[0] == 1 && dw.t->stride[1] == o.k))))) {
+        (dw && (dw.t->shape != shape || (turned && !(dw.t->stride.size() == 2 && dw.t->stride[0] == 1 && dw.t->stride[1] == o.k))))) {
         PyErr_SetString(PyExc_ValueError, "dx and dbias must be contiguous, dw contiguous or the transposing view of a contiguous [N, K]");
         return nullptr;
     }

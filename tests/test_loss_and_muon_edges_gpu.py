@@ -44,3 +44,20 @@ def test_the_layout_of_dw_is_its_strides(F, rows, layout):
         assert got[1].shape == (64, 500)
         # (of either layout the sums are the same up to their order: 300 terms)
         assert float((got[1].torch_view() - want[1].torch_view()).abs().max()) <= 1e-5 * float(want[1].torch_view().abs().max())
+
+
+def test_strides_that_are_not_given(F):
+    """A view with fewer strides than dims: those left out are 0, for dw's layout as for what the kernels read; as a given dw it is refused."""
+    x, column = torch.randn(6, 8, device="cuda"), torch.randn(8, device="cuda")
+    t = torch.zeros(6, dtype=torch.int64, device="cuda")
+    w = F.DeviceTensor(column, (8, 10), (1, 8))
+    w.strides = (1,)
+    one = tensor(F, torch.ones(1, device="cuda"))
+    loss, lse = F.linear_cross_entropy(tensor(F, x), w, t)
+    dx, dw = F.linear_cross_entropy_backward(one, tensor(F, x), w, t, lse)
+    assert dw.strides == (10, 1) and abs(float(loss.numpy()[0]) - np.log(10)) <= 1e-6
+    short = F.DeviceTensor(torch.empty(80, device="cuda"), (8, 10), (1, 8))
+    short.strides = (1,)
+    with pytest.raises(ValueError, match="dw contiguous or the transposing view"):
+        F.linear_cross_entropy_backward(one, tensor(F, x), w, t, lse, dw=short)
+    F.device_status()
