@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <exception>
 #include <initializer_list>
 #include <iterator>
 #include <map>
@@ -1832,6 +1833,18 @@ int with_scratch(uint32_t flags, void *stream, Body body) {
     return rc;
 }
 
+// An entry point's body: no C++ exception (of the host's memory) leaves the library, where it would end the caller's process.
+template <class Body>
+int no_exceptions(Body body) {
+    try {
+        return body();
+    } catch (const std::exception &e) {
+        return fail(MNI_B200_ERR_WORKSPACE, "host memory: %s", e.what());
+    } catch (...) {
+        return fail(MNI_B200_ERR_WORKSPACE, "the host side of the call failed");
+    }
+}
+
 }  // namespace
 
 int device_sm_count() {
@@ -2111,110 +2124,118 @@ int mni_b200_clip_and_step(int64_t count, float *const *params, float *const *ms
 
 int mni_b200_linear_cross_entropy_fwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias, const void *targets,
                                       int target_bytes, int reduction, float *loss, float *lse, uint32_t flags, void *stream) {
-    LossCall l;
-    int rc = check_loss(x, w, bias, targets, target_bytes, reduction, l);
-    if (rc) return rc;
-    if (flags != 0) return fail(MNI_B200_ERR_ARG, "flags 0x%x are not taken here", flags);
-    if ((l.M > 0 && !lse) || ((l.M > 0 || reduction != MNI_B200_REDUCE_NONE) && !loss)) return fail(MNI_B200_ERR_ARG, "loss or lse is null");
-    if (l.M == 0 && reduction != MNI_B200_REDUCE_NONE) {
-        DeviceState *st = nullptr;
-        rc = device_state(&st);
+    return no_exceptions([&]() -> int {
+        LossCall l;
+        int rc = check_loss(x, w, bias, targets, target_bytes, reduction, l);
         if (rc) return rc;
-        // the sum over no rows; as a mean 0 / 0 (an f32 of all ones is a NaN)
-        MNI_CUDA(cudaMemsetAsync(loss, reduction == MNI_B200_REDUCE_MEAN ? 0xff : 0, sizeof(float), static_cast<cudaStream_t>(stream)));
-        return MNI_B200_OK;
-    }
-    return with_scratch(flags, stream, [&](Call &call) { return loss_fwd_body(call, l, loss, lse); });
+        if (flags != 0) return fail(MNI_B200_ERR_ARG, "flags 0x%x are not taken here", flags);
+        if ((l.M > 0 && !lse) || ((l.M > 0 || reduction != MNI_B200_REDUCE_NONE) && !loss)) return fail(MNI_B200_ERR_ARG, "loss or lse is null");
+        if (l.M == 0 && reduction != MNI_B200_REDUCE_NONE) {
+            DeviceState *st = nullptr;
+            rc = device_state(&st);
+            if (rc) return rc;
+            // the sum over no rows; as a mean 0 / 0 (an f32 of all ones is a NaN)
+            MNI_CUDA(cudaMemsetAsync(loss, reduction == MNI_B200_REDUCE_MEAN ? 0xff : 0, sizeof(float), static_cast<cudaStream_t>(stream)));
+            return MNI_B200_OK;
+        }
+        return with_scratch(flags, stream, [&](Call &call) { return loss_fwd_body(call, l, loss, lse); });
+    });
 }
 
 int mni_b200_linear_cross_entropy_bwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias, const void *targets,
                                       int target_bytes, int reduction, const float *lse, const float *grad, float *dx, float *dw,
                                       float *dbias, uint32_t flags, void *stream) {
-    LossCall l;
-    int rc = check_loss(x, w, bias, targets, target_bytes, reduction, l);
-    if (rc) return rc;
-    constexpr uint32_t kTaken = MNI_B200_ACCUMULATE_DA | MNI_B200_ACCUMULATE_DB | MNI_B200_ACCUMULATE_DBIAS | MNI_B200_DB_TRANSPOSED;
-    if ((flags & ~kTaken) != 0) return fail(MNI_B200_ERR_ARG, "flags 0x%x are not taken here", flags & ~kTaken);
-    if (l.M > 0 && (!lse || !grad)) return fail(MNI_B200_ERR_ARG, "lse or grad is null");
-    return with_scratch(flags, stream, [&](Call &call) { return loss_bwd_body(call, l, lse, grad, dx, dw, dbias); });
+    return no_exceptions([&]() -> int {
+        LossCall l;
+        int rc = check_loss(x, w, bias, targets, target_bytes, reduction, l);
+        if (rc) return rc;
+        constexpr uint32_t kTaken = MNI_B200_ACCUMULATE_DA | MNI_B200_ACCUMULATE_DB | MNI_B200_ACCUMULATE_DBIAS | MNI_B200_DB_TRANSPOSED;
+        if ((flags & ~kTaken) != 0) return fail(MNI_B200_ERR_ARG, "flags 0x%x are not taken here", flags & ~kTaken);
+        if (l.M > 0 && (!lse || !grad)) return fail(MNI_B200_ERR_ARG, "lse or grad is null");
+        return with_scratch(flags, stream, [&](Call &call) { return loss_bwd_body(call, l, lse, grad, dx, dw, dbias); });
+    });
 }
 
 int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float a, float b, float c, float eps, void *stream) {
-    int rc = check_view(g, "g", 2);
-    if (rc) return rc;
-    NewtonSchulz ns;
-    std::vector<StepScales> scales;
-    rc = check_newton_schulz(steps, a, b, c, eps, ns, scales);
-    if (rc) return rc;
-    const int64_t rows = g->shape[g->ndim - 2], cols = g->shape[g->ndim - 1], batch = prod(g->shape, g->ndim - 2);
-    rc = check_matrix(rows, cols);
-    if (rc) return rc;
-    if (batch * rows * cols == 0) return MNI_B200_OK;
-    if (batch > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "more than 2^31-1 matrices");
-    if (!out) return fail(MNI_B200_ERR_ARG, "out is null");
-    return with_scratch(0, stream, [&](Call &call) -> int {
-        const float *src = g->ptr;
-        bool packed = true;
-        int64_t acc = 1;
-        for (int d = g->ndim - 1; d >= 0; --d) {
-            packed = packed && (g->shape[d] == 1 || g->stride[d] == acc);
-            acc *= g->shape[d];
-        }
-        if (!packed) {                             // into `out`, which is normalised in place
-            if (!call.dry()) {
-                const GatherView job{g, out, cols};
-                const int r = launch_gather(&job, 1, call.stream);
-                if (r) return r;
+    return no_exceptions([&]() -> int {
+        int rc = check_view(g, "g", 2);
+        if (rc) return rc;
+        NewtonSchulz ns;
+        std::vector<StepScales> scales;
+        rc = check_newton_schulz(steps, a, b, c, eps, ns, scales);
+        if (rc) return rc;
+        const int64_t rows = g->shape[g->ndim - 2], cols = g->shape[g->ndim - 1], batch = prod(g->shape, g->ndim - 2);
+        rc = check_matrix(rows, cols);
+        if (rc) return rc;
+        if (batch * rows * cols == 0) return MNI_B200_OK;
+        if (batch > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "more than 2^31-1 matrices");
+        if (!out) return fail(MNI_B200_ERR_ARG, "out is null");
+        return with_scratch(0, stream, [&](Call &call) -> int {
+            const float *src = g->ptr;
+            bool packed = true;
+            int64_t acc = 1;
+            for (int d = g->ndim - 1; d >= 0; --d) {
+                packed = packed && (g->shape[d] == 1 || g->stride[d] == acc);
+                acc *= g->shape[d];
             }
-            src = out;
-        }
-        std::vector<MuonEntry> e;
-        for (int64_t i = 0; i < batch; ++i)
-            e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, nullptr, 0, 0, rows, cols, rows * cols, 0.f});
-        return muon_body(call, e, ns, scales, 0.f, false, eps, 1.f);
+            if (!packed) {                             // into `out`, which is normalised in place
+                if (!call.dry()) {
+                    const GatherView job{g, out, cols};
+                    const int r = launch_gather(&job, 1, call.stream);
+                    if (r) return r;
+                }
+                src = out;
+            }
+            std::vector<MuonEntry> e;
+            for (int64_t i = 0; i < batch; ++i)
+                e.push_back(MuonEntry{nullptr, nullptr, src + i * rows * cols, out + i * rows * cols, nullptr, 0, 0, rows, cols, rows * cols, 0.f});
+            return muon_body(call, e, ns, scales, 0.f, false, eps, 1.f);
+        });
     });
 }
 
 int mni_b200_muon_step(int64_t count, float *const *params, float *const *momenta, const float *const *grads, const int64_t *rows,
                        const int64_t *cols, const float *scales, float lr, float momentum, int nesterov, float weight_decay, int steps,
                        float a, float b, float c, float eps, void *stream) {
-    if (count < 0) return fail(MNI_B200_ERR_ARG, "negative count");
-    if (count > 0 && (!params || !momenta || !grads || !rows || !cols || !scales)) return fail(MNI_B200_ERR_ARG, "null pointer");
-    NewtonSchulz ns;
-    std::vector<StepScales> bounds;
-    int rc = check_newton_schulz(steps, a, b, c, eps, ns, bounds);
-    if (rc) return rc;
-    std::vector<MuonEntry> e;
-    for (int64_t i = 0; i < count; ++i) {
-        rc = check_matrix(rows[i], cols[i]);
+    return no_exceptions([&]() -> int {
+        if (count < 0) return fail(MNI_B200_ERR_ARG, "negative count");
+        if (count > 0 && (!params || !momenta || !grads || !rows || !cols || !scales)) return fail(MNI_B200_ERR_ARG, "null pointer");
+        NewtonSchulz ns;
+        std::vector<StepScales> bounds;
+        int rc = check_newton_schulz(steps, a, b, c, eps, ns, bounds);
         if (rc) return rc;
-        const int64_t n = rows[i] * cols[i];
-        if (n == 0) continue;
-        if (!params[i] || !momenta[i] || !grads[i]) return fail(MNI_B200_ERR_ARG, "null pointer");
-        if (share_memory(params[i], momenta[i], n) || share_memory(params[i], grads[i], n) || share_memory(momenta[i], grads[i], n))
-            return fail(MNI_B200_ERR_ARG, "entry %lld: param, momentum and grad share memory", (long long)i);
-        e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, nullptr, 0, 0, rows[i], cols[i], n, lr * scales[i]});
-    }
-    // Entries that share memory with one before them begin another round, which starts from what that one left.
-    for (size_t first = 0; first < e.size();) {
-        Touched written, read;
-        size_t end = first;
-        for (; end < e.size(); ++end) {
-            const MuonEntry &m = e[end];
-            if (written.meets(m.param, m.n) || written.meets(m.momentum, m.n) || written.meets(m.grad, m.n) || read.meets(m.param, m.n) ||
-                read.meets(m.momentum, m.n))
-                break;
-            written.add(m.param, m.n);
-            written.add(m.momentum, m.n);
-            read.add(m.grad, m.n);
+        std::vector<MuonEntry> e;
+        for (int64_t i = 0; i < count; ++i) {
+            rc = check_matrix(rows[i], cols[i]);
+            if (rc) return rc;
+            const int64_t n = rows[i] * cols[i];
+            if (n == 0) continue;
+            if (!params[i] || !momenta[i] || !grads[i]) return fail(MNI_B200_ERR_ARG, "null pointer");
+            if (share_memory(params[i], momenta[i], n) || share_memory(params[i], grads[i], n) || share_memory(momenta[i], grads[i], n))
+                return fail(MNI_B200_ERR_ARG, "entry %lld: param, momentum and grad share memory", (long long)i);
+            e.push_back(MuonEntry{params[i], momenta[i], grads[i], nullptr, nullptr, 0, 0, rows[i], cols[i], n, lr * scales[i]});
         }
-        const std::vector<MuonEntry> round(e.begin() + first, e.begin() + end);
-        rc = with_scratch(0, stream,
-                          [&](Call &call) { return muon_body(call, round, ns, bounds, momentum, nesterov != 0, eps, 1.f - lr * weight_decay); });
-        if (rc) return rc;
-        first = end;
-    }
-    return MNI_B200_OK;
+        // Entries that share memory with one before them begin another round, which starts from what that one left.
+        for (size_t first = 0; first < e.size();) {
+            Touched written, read;
+            size_t end = first;
+            for (; end < e.size(); ++end) {
+                const MuonEntry &m = e[end];
+                if (written.meets(m.param, m.n) || written.meets(m.momentum, m.n) || written.meets(m.grad, m.n) || read.meets(m.param, m.n) ||
+                    read.meets(m.momentum, m.n))
+                    break;
+                written.add(m.param, m.n);
+                written.add(m.momentum, m.n);
+                read.add(m.grad, m.n);
+            }
+            const std::vector<MuonEntry> round(e.begin() + first, e.begin() + end);
+            rc = with_scratch(0, stream,
+                              [&](Call &call) { return muon_body(call, round, ns, bounds, momentum, nesterov != 0, eps, 1.f - lr * weight_decay); });
+            if (rc) return rc;
+            first = end;
+        }
+        return MNI_B200_OK;
+    });
 }
 
 int mni_b200_contiguous(const mni_b200_view *src, float *dst, void *stream) {

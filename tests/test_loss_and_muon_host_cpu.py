@@ -49,3 +49,26 @@ def test_nothing_is_added_to_memory_that_was_not_given(flag, wanted):
     from framework_b200 import _lib, ops
     with pytest.raises(ValueError, match=f"flags add to {wanted}, and none is given"):
         ops.linear_cross_entropy_backward(tensor((1,)), tensor(X), tensor(W), targets(), tensor(ROWS), flags=getattr(_lib, flag), want_dbias=True)
+
+
+def test_host_memory_that_runs_out_is_an_error():
+    """A list of half a million matrices, in a process that may have no more memory than it has: a status, and the process goes on."""
+    import os
+    import subprocess
+    import sys
+    program = """
+import ctypes as C, resource
+from framework_b200 import _lib
+lib, n = _lib.lib(), 1 << 19
+def pointers(base):
+    return (C.c_void_p * n)(*range(base, base + 1024 * n, 1024))
+lists = [pointers(1 << (40 + k)) for k in range(3)]
+four, ones = (C.c_int64 * n)(*([4] * n)), (C.c_float * n)()
+used = int(next(l for l in open("/proc/self/status") if l.startswith("VmSize")).split()[1]) * 1024
+resource.setrlimit(resource.RLIMIT_AS, (used + (8 << 20), resource.RLIM_INFINITY))
+status = lib.mni_b200_muon_step(n, *lists, four, four, ones, 0.1, 0.9, 1, 0.0, 5, 3.4445, -4.775, 2.0315, 1e-7, None)
+print(status, lib.mni_b200_last_error().decode())
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0 and done.stdout.startswith("7 host memory"), done.stdout + done.stderr[-1000:]
