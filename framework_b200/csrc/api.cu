@@ -1281,6 +1281,12 @@ int check_loss(const mni_b200_view *x, const mni_b200_view *w, const float *bias
         if (x->shape[d] != 0 && l.M > 0x7fffffffLL / x->shape[d]) return fail(MNI_B200_ERR_TOO_LARGE, "more than 2^31-1 rows");
         l.M *= x->shape[d];
     }
+    // The kernels' int32 row and column indices, to the end of a tile; and byte counts, which views of stride 0 could take past 64 bits.
+    constexpr int64_t kMost = 0x7fffffffLL - 4096;
+    constexpr double kMostElements = 1099511627776.0;                      // 2^40
+    if (l.M > kMost || l.N > kMost || l.K > kMost || static_cast<double>(l.M) * static_cast<double>(l.K) > kMostElements ||
+        static_cast<double>(l.K) * static_cast<double>(l.N) > kMostElements)
+        return fail(MNI_B200_ERR_TOO_LARGE, "%lld rows of %lld features for %lld classes are too many", (long long)l.M, (long long)l.K, (long long)l.N);
     if (target_bytes != 4 && target_bytes != 8) return fail(MNI_B200_ERR_ARG, "targets of %d bytes: 4 or 8 are taken", target_bytes);
     if (reduction < MNI_B200_REDUCE_NONE || reduction > MNI_B200_REDUCE_MEAN) return fail(MNI_B200_ERR_ARG, "unknown reduction %d", reduction);
     if (l.M > 0 && !targets) return fail(MNI_B200_ERR_ARG, "targets is null");
@@ -1336,7 +1342,9 @@ RowsIn rows_in(const LossCall &l) {
 // Few rows, or few logits: products in f32 as the other entry points make them, logits in scratch.  Otherwise from 16-bit planes, logits
 // never in memory.
 constexpr int64_t kLossRows = 8;
-bool loss_from_planes(const LossCall &l) { return l.M > kLossRows && l.M * l.N * l.K > kTinyWork; }
+bool loss_from_planes(const LossCall &l) {
+    return l.M > kLossRows && static_cast<double>(l.M) * static_cast<double>(l.N) * static_cast<double>(l.K) > kTinyWork;
+}
 
 float *dry_pointer() { return reinterpret_cast<float *>(static_cast<uintptr_t>(256)); }
 

@@ -232,6 +232,7 @@ MNI_B200_API int mni_b200_clip_and_step(int64_t count, float *const *params, flo
  * whatever its row of x holds.  One of N or more makes the row's loss NaN, and with it the gradients.
  * `reduction`: NONE leaves M losses in `loss`; SUM and MEAN one number, MEAN over the rows that are not left out (NaN where there
  * is none).  `lse` takes M numbers (those of rows left out too), which the backward needs.
+ * M, N and K are 2^31 - 4097 at most, x and w 2^40 elements, broadcast ones counted.
  *
  * Scratch, which mni_b200_workspace_query does not cover: 6 bytes an element of x and w and a pair (8 bytes) for every row and 64 classes; the
  * backward 6 bytes an element of x, w and a copy of x, that copy, dx once more, and 6 bytes a logit of as many classes as 384 MB hold.  Calls of up to 8

@@ -72,3 +72,17 @@ print(status, lib.mni_b200_last_error().decode())
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=120)
     assert done.returncode == 0 and done.stdout.startswith("7 host memory"), done.stdout + done.stderr[-1000:]
+
+
+LONG = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("rows,k,n", [(LONG, 1, 4), (4, 1, LONG), (4, LONG, 1), (1 << 21, 1 << 20, 4), (LONG - 5000, LONG - 5000, 1), (9, 1 << 20, 1 << 21)])
+def test_sizes_beyond_the_kernels_indices_are_refused(rows, k, n):
+    """Views of stride 0 have any extent without the memory; what the call would need in scratch goes past 64 bits."""
+    from framework_b200 import _lib
+    lib = _lib.lib()
+    x, w = _lib.make_view(256, (rows, k), (0, 0)), _lib.make_view(256, (k, n), (0, 0))
+    assert lib.mni_b200_linear_cross_entropy_fwd(x, w, None, 512, 8, 2, 512, 512, 0, None) == 9
+    assert "too many" in lib.mni_b200_last_error().decode()
+    assert lib.mni_b200_linear_cross_entropy_bwd(x, w, None, 512, 8, 2, 512, 512, 512, 512, None, 0, None) == 9
