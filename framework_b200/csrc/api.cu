@@ -1792,9 +1792,9 @@ int check_newton_schulz(int steps, float a, float b, float c, float eps, NewtonS
     ns = NewtonSchulz{steps, a, b, c};
     return step_scales(ns, scales);
 }
-int check_matrix(int64_t rows, int64_t cols) {
+int check_matrix(int64_t rows, int64_t cols, int steps) {
     if (rows < 0 || cols < 0) return fail(MNI_B200_ERR_ARG, "negative extent");
-    if (rows > 0x7fffffffLL || cols > 0x7fffffffLL || (rows > 0 && cols > (1LL << 38) / rows))
+    if (rows > 0x7fffffffLL || cols > 0x7fffffffLL || (rows > 0 && cols > (1LL << 38) / rows) || (steps > 0 && std::max(rows, cols) > kNewtonLongest))
         return fail(MNI_B200_ERR_TOO_LARGE, "a matrix of %lld x %lld is too large", (long long)rows, (long long)cols);
     return MNI_B200_OK;
 }
@@ -2173,7 +2173,7 @@ int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float 
         rc = check_newton_schulz(steps, a, b, c, eps, ns, scales);
         if (rc) return rc;
         const int64_t rows = g->shape[g->ndim - 2], cols = g->shape[g->ndim - 1], batch = prod(g->shape, g->ndim - 2);
-        rc = check_matrix(rows, cols);
+        rc = check_matrix(rows, cols, steps);
         if (rc) return rc;
         if (batch * rows * cols == 0) return MNI_B200_OK;
         if (batch > 0x7fffffffLL) return fail(MNI_B200_ERR_TOO_LARGE, "more than 2^31-1 matrices");
@@ -2214,7 +2214,7 @@ int mni_b200_muon_step(int64_t count, float *const *params, float *const *moment
         if (rc) return rc;
         std::vector<MuonEntry> e;
         for (int64_t i = 0; i < count; ++i) {
-            rc = check_matrix(rows[i], cols[i]);
+            rc = check_matrix(rows[i], cols[i], steps);
             if (rc) return rc;
             const int64_t n = rows[i] * cols[i];
             if (n == 0) continue;

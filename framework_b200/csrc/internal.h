@@ -413,6 +413,8 @@ struct NewtonProblem {
 struct NewtonStep {
     float a, r, r_diagonal, q, q_diagonal, x;
 };
+// The longer side of a matrix: one tile's contraction over it, which others wait for, takes less than half of what any wait may (24.4 clocks an element).
+constexpr int64_t kNewtonLongest = 1 << 26;
 constexpr int kNewtonGroups = 8, kNewtonMatrices = 512, kNewtonSteps = 100;      // of a launch (25 KB of kernel parameters)
 // out[i] = x of matrix i, or (update) decay * out[i] - scale[i] * x.  counters: 1 + 3 * matrices words, zero.
 int launch_newton_schulz(const NewtonProblem *problems, int count, const NewtonStep *steps, int step_count, float *const *out, const float *scale, bool update,

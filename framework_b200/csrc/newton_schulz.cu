@@ -47,6 +47,7 @@ constexpr int kThreads = 32 * (4 + kEpiWarps);
 constexpr int kLaunchRegs = 168;                   // a thread has at launch; launch() checks that the compiler took no fewer
 constexpr int kIssueRegs = 56, kEpiRegs = 224;
 static_assert(kThreads * kLaunchRegs <= 65536 && kIssueRegs + 2 * kEpiRegs <= 3 * kLaunchRegs, "more registers than the launch has");
+static_assert(2 * 25 * kNewtonLongest <= kWaitCycles, "a wait for one tile may run out");
 constexpr int kBars = 3 * kStagesMax + 4 + 2 * kRing + 1;
 constexpr int kFixedSmem = 1024 + kEpiWarps * kPatchBytes + kBars * 8 + 64;
 

@@ -86,3 +86,18 @@ def test_sizes_beyond_the_kernels_indices_are_refused(rows, k, n):
     assert lib.mni_b200_linear_cross_entropy_fwd(x, w, None, 512, 8, 2, 512, 512, 0, None) == 9
     assert "too many" in lib.mni_b200_last_error().decode()
     assert lib.mni_b200_linear_cross_entropy_bwd(x, w, None, 512, 8, 2, 512, 512, 512, 512, None, 0, None) == 9
+
+
+def test_matrices_whose_tiles_outlast_a_wait_are_refused():
+    """A tile's contraction over 2^27 elements takes longer than the tiles behind it may wait."""
+    import ctypes as C
+
+    from framework_b200 import _lib
+    lib = _lib.lib()
+    newton = (3.4445, -4.775, 2.0315, 1e-7)
+    for rows, cols in ((4, (1 << 26) + 1), ((1 << 26) + 1, 4), (1, LONG)):
+        assert lib.mni_b200_orthogonalize(_lib.make_view(256, (rows, cols), (0, 0)), 512, 5, *newton, None) == 9
+        assert "too large" in lib.mni_b200_last_error().decode()
+        one = [(C.c_void_p * 1)(1 << (40 + k)) for k in range(3)]
+        sizes = (C.c_int64 * 1)(rows), (C.c_int64 * 1)(cols)
+        assert lib.mni_b200_muon_step(1, *one, *sizes, (C.c_float * 1)(1.0), 0.1, 0.9, 1, 0.0, 5, *newton, None) == 9
