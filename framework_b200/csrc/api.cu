@@ -2172,6 +2172,9 @@ int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float 
         std::vector<StepScales> scales;
         rc = check_newton_schulz(steps, a, b, c, eps, ns, scales);
         if (rc) return rc;
+        double most = 1.0;                         // (views of stride 0 could take the product past 64 bits)
+        for (int d = 0; d < g->ndim; ++d) most *= static_cast<double>(std::max<int64_t>(g->shape[d], 1));
+        if (most > 1099511627776.0) return fail(MNI_B200_ERR_TOO_LARGE, "g has too many elements: more than 2^40");
         const int64_t rows = g->shape[g->ndim - 2], cols = g->shape[g->ndim - 1], batch = prod(g->shape, g->ndim - 2);
         rc = check_matrix(rows, cols, steps);
         if (rc) return rc;

@@ -101,3 +101,12 @@ def test_matrices_whose_tiles_outlast_a_wait_are_refused():
         one = [(C.c_void_p * 1)(1 << (40 + k)) for k in range(3)]
         sizes = (C.c_int64 * 1)(rows), (C.c_int64 * 1)(cols)
         assert lib.mni_b200_muon_step(1, *one, *sizes, (C.c_float * 1)(1.0), 0.1, 0.9, 1, 0.0, 5, *newton, None) == 9
+
+
+def test_batches_whose_count_does_not_fit_are_refused():
+    from framework_b200 import _lib
+    lib = _lib.lib()
+    for lead in ((1 << 30, 1 << 30, 1 << 4), (1 << 30, 1 << 20)):               # 2^64 matrices, which are none in 64 bits; 2^50
+        g = _lib.make_view(256, (*lead, 4, 4), (0,) * (len(lead) + 2))
+        assert lib.mni_b200_orthogonalize(g, 512, 5, 3.4445, -4.775, 2.0315, 1e-7, None) == 9
+        assert "too many elements" in lib.mni_b200_last_error().decode()
