@@ -412,6 +412,7 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                     }
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
+                    __syncwarp();                  // what lane 0 has acquired is every lane's (the vote orders no memory)
                     asm volatile("fence.proxy.async;" ::: "memory");       // their stores before the copies of whichever lane issues them
                 }
                 const int blocks = (contraction(t) + BK - 1) / BK, parity = t.step & 1;
