@@ -2652,7 +2652,7 @@ static FusedTiling fused_tiling(const GemmProblem &p, int sm_count) {
         t.lone = lone;
         t.tiles_m = (p.M + side - 1) / side;
         t.tiles_n = (p.N + side - 1) / side;
-        t.units = p.batch * t.tiles_m * t.tiles_n;
+        t.units = t.tiles_m * t.tiles_n;
         t.slots = lone ? sm_count : std::max(1, sm_count / 2);
         return t;
     };
@@ -2668,11 +2668,11 @@ int fused_stretch(const GemmProblem &p, int sm_count) { return fused_tiling(p, s
 
 // A product from 16-bit planes with one of the fused epilogues: whole tiles, dealt out round-robin.
 int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, uint32_t *err_word, int sm_count, cudaStream_t stream) {
-    if (p.M <= 0 || p.N <= 0 || p.batch <= 0) return MNI_B200_OK;
+    if (p.batch != 1) return fail(MNI_B200_ERR_ARG, "internal: fused epilogues take one product, not a batch of %lld", (long long)p.batch);
+    if (p.M <= 0 || p.N <= 0) return MNI_B200_OK;
     const FusedTiling t = fused_tiling(p, sm_count);
-    if (p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.K > 0x7fffffffLL || p.batch > 0x7fffffffLL || t.tiles_m * t.tiles_n > 0x3fffffffLL / p.batch)
-        return fail(MNI_B200_ERR_TOO_LARGE, "product %lld x %lld x %lld (batch %lld) exceeds the kernels' int32 indexing", (long long)p.M,
-                    (long long)p.N, (long long)p.K, (long long)p.batch);
+    if (p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.K > 0x7fffffffLL || t.units > 0x3fffffffLL)
+        return fail(MNI_B200_ERR_TOO_LARGE, "product %lld x %lld x %lld exceeds the kernels' int32 indexing", (long long)p.M, (long long)p.N, (long long)p.K);
     Plan pl{};
     pl.bn = t.lone ? 128 : 256;
     pl.bk = 64;

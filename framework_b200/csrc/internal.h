@@ -213,11 +213,11 @@ struct FusedArgs {
     float2 *pairs;                 // [stretch of columns][row]
     float *at_target;              // [row]
     const float *lse;
-    // planes written: [batch][row][pitch], `matrix` and `plane` elements apart
+    // planes written: [row][pitch], `plane` elements apart
     uint16_t *dst;
-    long long dst_pitch, dst_matrix, dst_plane;
+    long long dst_pitch, dst_plane;
 };
-// Columns that a pair of launch_gemm_fused stands for.
+// Columns that a pair of launch_gemm_fused stands for.  (One product: the epilogues know no batch.)
 int fused_stretch(const GemmProblem &p, int sm_count);
 int launch_gemm_fused(const GemmProblem &p, FusedKind kind, const FusedArgs &f, uint32_t *err_word, int sm_count, cudaStream_t stream);
 constexpr int kGradExponent = 14;      // logit gradients, -1 to 1, are multiplied by 2^14 in f16 planes
