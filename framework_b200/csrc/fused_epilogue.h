@@ -9,8 +9,16 @@
 // The kernel calls them chunk after chunk in a loop that is not unrolled, and moves the registers down in between: unrolled over 128
 // columns their code (40 KB, executed once a tile) came from beyond the instruction caches, and a tile's epilogue took 12 us.
 //
-// Planes are written row by row, 32 bytes a store of one thread: whole sectors.  The scale is fixed, not looked for: a gradient of
-// logits is at most one.
+// Planes are written row by row, 32 bytes a store of one thread: whole sectors.  The scale of f16 planes is fixed, 2^14, not looked for: a
+// gradient d of logits is at most one.  So hi is subnormal below 2^-28, where the two planes begin to hold fewer than 22 bits, and nothing is left
+// below 2^-51; with the lo * lo that products leave out, what a product takes of a d is off by an absolute 2^-50 (a row's weight is not in d
+// yet).  A class of probability 1e-10 in every row has dw and dbias to 1e-5 of their size, one of 1e-13 to 1e-2.  It is a choice: beside what the
+// row's own target adds (1 - p) it is 2^-50 of the row's gradient, and three bf16 planes, which would keep f32's range, are six products for three.
+// Nor is their range looked at as an operand's is (half.cu): most classes are improbable in most rows, so that most calls would take six.
+//
+// exp: ex2.approx of the argument times log2(e).  That product's rounding makes a term off by (max - z) 2^-24 of itself at most, either way; a row's sum
+// averages it over its terms, and the logits' own error (1e-6 of what they are summed from) is more.  In d it would be the result's, and is
+// carried along.
 #pragma once
 
 #include <cuda_fp16.h>

@@ -249,6 +249,10 @@ MNI_B200_API int mni_b200_linear_cross_entropy_fwd(const mni_b200_view *x, const
  * Its backward, from the forward's operands and `lse`.  `grad` is the gradient of `loss`: M numbers for NONE, else one.  dx takes x's
  * shape and dw [K, N] (with MNI_B200_DB_TRANSPOSED laid out [N, K], for a weight stored so), contiguous; dbias N numbers.
  * Each may be NULL.  The ACCUMULATE flags of mni_b200_matmul_bwd (DA: dx, DB: dw) add instead of overwriting.
+ *
+ * Calls of more than 8 rows and 2^23 multiply-adds take logits' gradients (before the rows' weights: exp(z - lse) - [class = target]) as 22 bits
+ * and an absolute 2^-50, unless x or w have a range that needs the planes of mni_b200_workspace_set that keep all bits.  So dw and dbias of a
+ * class whose probability is below 2^-28 in every row have fewer bits than an f32 holds, and none of probabilities below 2^-51.
  */
 MNI_B200_API int mni_b200_linear_cross_entropy_bwd(const mni_b200_view *x, const mni_b200_view *w, const float *bias,
                                                    const void *targets, int target_bytes, int reduction, const float *lse,
