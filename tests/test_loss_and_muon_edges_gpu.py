@@ -61,3 +61,43 @@ def test_strides_that_are_not_given(F):
     with pytest.raises(ValueError, match="dw contiguous or the transposing view"):
         F.linear_cross_entropy_backward(one, tensor(F, x), w, t, lse, dw=short)
     F.device_status()
+
+
+@pytest.mark.parametrize("shape", [(64, 8192), (8192, 64), (100, 5000), (5003, 101), (3, 12000), (128, 4096), (1, 100000), (100000, 1)])
+def test_thin_matrices(F, shape):
+    """A short side and thousands on the other: one or a few tiles whose contraction is the long side."""
+    from test_muon_gpu import close, gradient, truth
+    g = gradient(sum(shape), *shape)
+    got = F.orthogonalize(tensor(F, g)).torch_view()
+    F.device_status()
+    close(got, *truth(g))
+
+
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+def test_updates_take_nothing_from_what_scratch_held(F, monkeypatch, tile):
+    """As for the loss: scratch full of NaN, ragged matrices, each tiling."""
+    import ctypes as C
+
+    from test_muon_gpu import gradient
+    monkeypatch.setenv("MNI_B200_NEWTON_TILE", tile)
+    shapes = [(33, 65), (1, 1), (130, 257), (257, 130), (300, 301), (2, 70, 45)]
+    start = [[gradient(7 * i + j, *s) for i, s in enumerate(shapes)] for j in range(3)]
+
+    def run():
+        ps, ms, gs = ([t.clone() for t in ts] for ts in start)
+        F.muon_step([tensor(F, t) for t in ps], [tensor(F, t) for t in ms], [tensor(F, t) for t in gs], lr=0.05)
+        out = [F.orthogonalize(tensor(F, g), steps=s).torch_view().clone() for g in gs for s in (0, 2)]
+        F.device_status()
+        return ps + ms + out
+    want = run()
+    size = 64 << 20
+    scratch = torch.full((size,), 0xff, dtype=torch.uint8, device="cuda")
+    lib = F._lib.lib()
+    F._lib.check(lib.mni_b200_workspace_set(C.c_void_p(scratch.data_ptr()), size))
+    try:
+        got = run()
+        torch.cuda.synchronize()
+    finally:
+        F._lib.check(lib.mni_b200_workspace_set(None, 0))
+    assert bool((scratch != 0xff).any())
+    assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(got, want))
