@@ -1340,7 +1340,20 @@ RowsIn rows_in(const LossCall &l) {
 }
 
 // Few rows, or few logits: products in f32 as the other entry points make them, logits in scratch.  Otherwise from 16-bit planes, logits
-// never in memory.
+// never in memory.  The limits are where the f32 entry points' forward stops to multiply in f32 (streams of up to 8 rows, one launch of up to
+// 2^23 multiply-adds) and takes three TF32 passes, whose logits are three to ten times further off than those of planes: the loss is a small
+// difference of theirs.  It is a choice against time, for beyond the limits f32 operands are faster up to 256 rows.  us forward / backward,
+// and relative 2-norm errors of losses and dx, from planes | from f32 operands (cold L2, medians of 15):
+//       8 x 1024 x 32000   104 / 212  7e-7 9e-7 |  50 / 109  6e-8 5e-6
+//       9 x 1024 x 32000   109 / 218  6e-7 7e-7 |  46 / 115  2e-6 5e-6
+//      16 x 1024 x 32000   109 / 208  6e-7 7e-7 |  48 / 117  8e-6 5e-6
+//      64 x 1024 x 32000   108 / 212  6e-7 7e-7 |  52 / 123  8e-6 5e-6
+//     128 x 1024 x 32000   113 / 218  7e-7 6e-7 |  65 / 168  8e-6 4e-6
+//     256 x 1024 x 32000   115 / 235  6e-7 6e-7 |  88 / 231  8e-6 5e-6
+//     256 x 256 x 8000      29 / 63             |  26 / 49
+//     128 x 64 x 1000       21 / 55   2e-7 4e-7 |  13 / 26   1e-7 9e-7       (2^23 multiply-adds and fewer: f32 FMAs)
+//     300 x 64 x 500        21 / 56   2e-7 4e-7 |  17 / 27   2e-6 1e-6       (more)
+//    1000 x 64 x 1000       22 / 53   2e-7 4e-7 |  17 / 31   2e-6 1e-6
 constexpr int64_t kLossRows = 8;
 bool loss_from_planes(const LossCall &l) {
     return l.M > kLossRows && static_cast<double>(l.M) * static_cast<double>(l.N) * static_cast<double>(l.K) > kTinyWork;
@@ -1480,7 +1493,8 @@ int loss_bwd_small(Call &c, const LossCall &l, const float *lse, const float *gr
     return rc;
 }
 
-// Classes of a piece of the backward: a multiple of 256.
+// Classes of a piece of the backward: a multiple of 256, as many as kPieceBytes of planes hold, and 256 where they hold fewer (more than 262144 rows:
+// 1536 bytes a row).
 constexpr int64_t kPieceBytes = 384ll << 20;
 int64_t piece_of(const LossCall &l) {
     const int64_t fits = std::max<int64_t>(256, kPieceBytes / (6 * l.M) / 256 * 256);

@@ -234,9 +234,12 @@ MNI_B200_API int mni_b200_clip_and_step(int64_t count, float *const *params, flo
  * is none).  `lse` takes M numbers (those of rows left out too), which the backward needs.
  * M, N and K are 2^31 - 4097 at most, x and w 2^40 elements, broadcast ones counted.
  *
- * Scratch, which mni_b200_workspace_query does not cover: 6 bytes an element of x and w and a pair (8 bytes) for every row and 64 classes; the
- * backward 6 bytes an element of x, w and a copy of x, that copy, dx once more, and 6 bytes a logit of as many classes as 384 MB hold.  Calls of up to 8
- * rows, or up to 2^23 multiply-adds, 4 bytes a logit.  A captured call is run once beforehand, as any other that cannot do without.
+ * Scratch, which mni_b200_workspace_query does not cover: 6 bytes an element of x and w (planes' rows padded to 64 elements) and a pair (8 bytes) for
+ * every row and 64 classes; the backward 6 bytes an element of x, w and a copy of x, that copy, dx once more, and 6 bytes a logit of as many
+ * classes as 384 MB hold, 256 at least (1536 bytes a row).  Calls of up to 8 rows, or up to 2^23 multiply-adds, 4 bytes a logit and what
+ * mni_b200_matmul_fwd and _bwd take for their products.  What products split over SMs add to that, up to a fifth in calls of some MB, goes by the
+ * device; a call that finds a caller's buffer too small says how much it needs (mni_b200_last_error).  A captured call is run once
+ * beforehand, as any other that cannot do without.
  */
 #define MNI_B200_REDUCE_NONE 0
 #define MNI_B200_REDUCE_SUM  1
