@@ -7,7 +7,7 @@
 // CTAs (pairs) draw them in that order from a counter; a unit waits until the units of its matrix's product before have been counted as
 // done.  It waits only for units of lower numbers, which have been drawn already, so the lowest unfinished one can always run.  So
 // products of different matrices, steps and shapes fill each other's gaps: as one launch for each product and shape, each waiting
-// for the one before, thirty matrices of 512 x 512 and 512 x 2048 took 1550 us, of which the pipe worked 260.
+// for the one before, thirty matrices of 512 x 512 and 512 x 2048 took 1290 us, of which the pipe worked 260.
 //
 //   warp 0, 1   TMA producers of A and of B (both wait for the unit's matrix, then order the other CTAs' stores before their copies)
 //   warp 2      issues the MMAs (of a pair: the leader's; the peer's draws the units)
@@ -25,8 +25,8 @@
 //
 // What bounds it.  One matrix: the chain of 15 products, each of which takes its contraction (16000 clocks at 768), 1200 for the first operands,
 // 700 for the accumulators, 2500 for the planes, 1500 until they are counted and 2000 until the others see that; 768 x 768 takes 203 us,
-// 64 x 32 68.  Many: thirty matrices of 512 x 512 and 512 x 2048 take 725 us, the pipe busy for 45 %, L2 at 8.1 TB/s, 1.2 GB from and to DRAM (their planes
-// are 220 MB, more than L2 holds): a tile of 512 elements takes 12500 clocks of the pipe and 10000 of its epilogue, during which the next tile's
+// 64 x 32 68.  Many: thirty matrices of 512 x 512 and 512 x 2048 take 725 us as a whole step in a loop.  This launch by itself is 570 of them, the
+// pipe busy for 45 %, L2 at 8.1 TB/s, 1.2 GB from and to DRAM (their planes are 220 MB, more than L2 holds): a tile of 512 elements takes 12500 clocks of the pipe and 10000 of its epilogue, during which the next tile's
 // accumulators can only fill once.
 #include "fused_epilogue.h"
 #include "internal.h"
