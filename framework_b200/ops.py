@@ -168,7 +168,8 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 def orthogonalize(g: DeviceTensor, *, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ,
                   eps: float = 1e-7) -> DeviceTensor:
     """Each matrix of g [.., rows, cols] divided by its Frobenius norm (+ eps), then ``steps`` times x <- a x + (b A + c A^2) x with
-    A = x x^T (from the right for more rows than columns): a matrix of the same singular vectors whose singular values are nearly one."""
+    A = x x^T (from the right for more rows than columns): a matrix of the same singular vectors whose singular values are nearly one.
+    Coefficients with which some singular value from 0 to 1 could pass 1e9 within the steps are refused."""
     a, b, c = coefficients
     return _host.orthogonalize(g, int(steps), a, b, c, eps)
 

@@ -267,6 +267,7 @@ MNI_B200_API int mni_b200_linear_cross_entropy_bwd(const mni_b200_view *x, const
  * x <- a x + (b A + c A^2) x with A = x x^T (from the right for matrices with more rows than columns).  g is [.., rows, cols] with any
  * strides, each of its matrices by itself; `out` is contiguous in its shape and may be g's own memory where g is contiguous.
  * Matrices are 2^38 elements at most, and with any step 2^26 on their longer side; g is 2^40 in all, broadcast ones counted.
+ * Coefficients are refused with which a singular value from 0 to 1 could pass 1e9 within the steps, whatever g holds.
  * (No counterpart in the reference.)
  */
 MNI_B200_API int mni_b200_orthogonalize(const mni_b200_view *g, float *out, int steps, float a, float b, float c, float eps,
