@@ -203,9 +203,8 @@ int scratch_base(DeviceState &st, size_t bytes, cudaStream_t stream, uint8_t **b
     }
     if (bytes > st.ws_bytes) {
         const size_t want = scratch_for(bytes);
-        // Growing frees the old buffer, which a capturing stream must not do (it would end the capture in
-        // an error).
-        if (st.ws && stream_is_capturing(stream))
+        // Allocating, and freeing the old buffer, would end a capture in an error.
+        if (stream_is_capturing(stream))
             return fail(MNI_B200_ERR_WORKSPACE,
                         "scratch would have to grow from %zu to %zu bytes while the stream is capturing: run the call "
                         "once before the capture, or hand the library a buffer (mni_b200_workspace_set)",

@@ -101,3 +101,55 @@ def test_updates_take_nothing_from_what_scratch_held(F, monkeypatch, tile):
         F._lib.check(lib.mni_b200_workspace_set(None, 0))
     assert bool((scratch != 0xff).any())
     assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("before", ["nothing", "a small call"])
+def test_a_first_call_that_is_captured_is_refused_and_the_capture_goes_on(F, before):
+    """Scratch cannot be allocated, nor grow, while a stream captures: nothing is recorded, and the capture stays valid."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    # (each needs more than the MB that the library's scratch is larger than a small call's)
+    x, w = torch.randn(300, 256, device="cuda", generator=gen), torch.randn(256, 2000, device="cuda", generator=gen)
+    t = torch.randint(0, 2000, (300,), device="cuda", generator=gen)
+    p, m, g = (torch.randn(400, 500, device="cuda", generator=gen) for _ in range(3))
+    one, lse = tensor(F, torch.ones(1, device="cuda")), tensor(F, torch.ones(300, device="cuda"))
+    tx, tw, tp, tm, tg = (tensor(F, v) for v in (x, w, p, m, g))
+    kept = p.clone(), m.clone()
+    F.device_status()
+    F._lib.check(F._lib.lib().mni_b200_release())
+    if before != "nothing":
+        F.linear_cross_entropy(tensor(F, x[:9, :4].contiguous()), tensor(F, w[:4, :5].contiguous()), t[:9] % 5)
+    stream = torch.cuda.Stream()
+    total = torch.zeros(1, device="cuda")
+    calls = (lambda: F.linear_cross_entropy(tx, tw, t), lambda: F.linear_cross_entropy_backward(one, tx, tw, t, lse), lambda: F.orthogonalize(tg),
+             lambda: F.muon_step([tp], [tm], [tg], lr=0.1))
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        launched = F.launch_count()
+        with torch.cuda.graph(graph, stream=stream):
+            for call in calls:
+                with pytest.raises(F._lib.MniError) as e:
+                    call()
+                assert e.value.status == 7 and "captur" in e.value.message, e.value
+            total += 1
+        assert F.launch_count() == launched
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(total) == 1.0 and torch.equal(p, kept[0]) and torch.equal(m, kept[1])
+    for call in calls:
+        call()
+    F.device_status()
+
+
+@pytest.mark.parametrize("rows", [6, 256])
+def test_features_seen_through_unusual_views(F, rows):
+    """One feature for all columns, extents of one with any stride, as many dims as a view may have."""
+    from test_linear_cross_entropy_gpu import compare, make
+    _, w, t, b = make(3, rows, 48, 700, bias=True)
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    compare(F, torch.randn(rows, 1, device="cuda", generator=gen).expand(rows, 48), w, t, b)
+    compare(F, torch.randn(1, 1, device="cuda", generator=gen).expand(rows, 48), w, t, b)
+    flat = torch.randn(rows, 48, device="cuda", generator=gen)
+    compare(F, flat.as_strided((1, rows, 1, 48), (7, 48, 1000003, 1)), w, t.reshape(1, rows, 1), b)
+    if rows == 256:
+        x = torch.randn(2, 2, 4, 2, 2, 2, 2, 96, device="cuda", generator=gen)[..., ::2].permute(3, 1, 0, 2, 6, 4, 5, 7)
+        compare(F, x, w, t.reshape(x.shape[:-1]), b)
