@@ -24,8 +24,8 @@
 // the large ones do twice as much a clock: tiling() weighs the two.
 //
 // What bounds it.  One matrix: the chain of 15 products, each of which takes its contraction (16000 clocks at 768), 1200 for the first operands,
-// 700 for the accumulators, 2500 for the planes, 1500 until they are counted and 2000 until the others see that; 768 x 768 takes 203 us,
-// 64 x 32 68.  Many: thirty matrices of 512 x 512 and 512 x 2048 take 725 us as a whole step in a loop.  This launch by itself is 570 of them, the
+// 700 for the accumulators, 2500 for the planes, 1500 until they are counted and 2000 until the others see that; 768 x 768 takes 201 us,
+// 64 x 32 62 to 66; of a thin one the long side is one contraction of one or a few tiles (128 x 4096 304, 64 x 8192 523).  Many: thirty matrices of 512 x 512 and 512 x 2048 take 725 us as a whole step in a loop.  This launch by itself is 570 of them, the
 // pipe busy for 45 %, L2 at 8.1 TB/s, 1.2 GB from and to DRAM (their planes are 220 MB, more than L2 holds): a tile of 512 elements takes 12500 clocks of the pipe and 10000 of its epilogue, during which the next tile's
 // accumulators can only fill once.
 #include "fused_epilogue.h"
@@ -395,24 +395,23 @@ newton_schulz_kernel(const __grid_constant__ Args p) {
                     const int before = t.product == 0 ? 2 : t.product - 1;
                     const unsigned tiles = static_cast<unsigned>(before == 2 ? g.tm3 * g.tn3 : g.tiles1);
                     const unsigned want = tiles * static_cast<unsigned>(t.product == 0 ? t.step : t.step + 1) * (CG * kEpiWarps);
-                    if (lane == 0) {
-                        const unsigned *const done = p.done + 3 * (g.first_matrix + t.matrix) + before;
-                        const long long t0 = clock64();
-                        while (true) {
-                            unsigned seen;
-                            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(done) : "memory");
-                            if (seen >= want) break;
-                            if (*abort_flag || clock64() - t0 > p.wait_cycles) {
-                                *abort_flag = 1u;
-                                atomicCAS(p.err, 0u, 0x800u | static_cast<unsigned>(t.product));
-                                ok = false;
-                                break;
-                            }
+                    // Every lane acquires the count itself, as any of them may issue the copies; the vote orders no memory.  (Lane 0 alone and a
+                    // __syncwarp: 768 x 768 207 us for 201.)
+                    const unsigned *const done = p.done + 3 * (g.first_matrix + t.matrix) + before;
+                    const long long t0 = clock64();
+                    while (true) {
+                        unsigned seen;
+                        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(done) : "memory");
+                        if (seen >= want) break;
+                        if (*abort_flag || clock64() - t0 > p.wait_cycles) {
+                            *abort_flag = 1u;
+                            atomicCAS(p.err, 0u, 0x800u | static_cast<unsigned>(t.product));
+                            ok = false;
+                            break;
                         }
                     }
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    __syncwarp();                  // what lane 0 has acquired is every lane's (the vote orders no memory)
                     asm volatile("fence.proxy.async;" ::: "memory");       // their stores before the copies of whichever lane issues them
                 }
                 const int blocks = (contraction(t) + BK - 1) / BK, parity = t.step & 1;
