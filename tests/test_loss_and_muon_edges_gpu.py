@@ -153,3 +153,49 @@ def test_features_seen_through_unusual_views(F, rows):
     if rows == 256:
         x = torch.randn(2, 2, 4, 2, 2, 2, 2, 96, device="cuda", generator=gen)[..., ::2].permute(3, 1, 0, 2, 6, 4, 5, 7)
         compare(F, x, w, t.reshape(x.shape[:-1]), b)
+
+
+@pytest.mark.parametrize("misalign", [1, 2])
+@pytest.mark.parametrize("layout", ["stored", "tied"])
+@pytest.mark.parametrize("rows,k,n", [(6, 32, 2000), (300, 101, 1003), (260, 128, 1024)])
+def test_everything_off_a_16_byte_boundary(F, rows, k, n, layout, misalign):
+    """Operands, bias, lse and gradients one or two floats behind a boundary, between guard zones."""
+    from conftest import Guarded
+    from test_linear_cross_entropy_gpu import close, make, truth
+
+    def moved(t):
+        flat = torch.empty(t.numel() + misalign, device="cuda")
+        flat[misalign:] = t.reshape(-1)
+        return flat[misalign:].view(t.shape)
+    x, w, t, b = make(1, rows, k, n, "stored", bias=True, masked=True)
+    x, b = moved(x), moved(b)
+    w = moved(w) if layout == "stored" else moved(w.t().contiguous()).t()
+    values, offs = truth(x, w, t, b, "mean", torch.ones(1, device="cuda"))
+    loss, lse = F.linear_cross_entropy(tensor(F, x), tensor(F, w), t, tensor(F, b))
+    outs = [Guarded(F, s, None, misalign) for s in ((rows, k), (n, k) if layout == "tied" else (k, n), (n,))]
+    dw = outs[1].tensor.permute([1, 0]) if layout == "tied" else outs[1].tensor
+    got = F.linear_cross_entropy_backward(tensor(F, moved(torch.ones(1, device="cuda"))), tensor(F, x), tensor(F, w), t, tensor(F, moved(lse.torch_view())),
+                                          tensor(F, b), want_dbias=True, dx=outs[0].tensor, dw=dw, dbias=outs[2].tensor)
+    F.device_status()
+    for i, o in enumerate(outs):
+        o.check(f"output {i}")
+    close(loss.torch_view(), values["loss"], offs["loss"], "loss")
+    for name, g in zip(("dx", "dw", "dbias"), got):
+        close(g.torch_view(), values[name], offs[name], name)
+
+
+@pytest.mark.parametrize("reserve", [60, 140])
+def test_beside_a_kernel_that_takes_the_other_sms(F, reserve):
+    """Grids of few CTAs, down to eight: tiles that wait for one another are drawn in an order in which the first can always run."""
+    from test_linear_cross_entropy_gpu import compare, make
+    from test_muon_gpu import close, gradient, truth
+    g = [gradient(3, 300, 260), gradient(4, 520, 700)]
+    F.sm_reserve(reserve)
+    try:
+        got = [F.orthogonalize(tensor(F, v)).torch_view() for v in g]
+        F.device_status()
+        compare(F, *make(5, 300, 128, 1500, bias=True, masked=True))
+    finally:
+        F.sm_reserve(0)
+    for v, a in zip(g, got):
+        close(a, *truth(v))
